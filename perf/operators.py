@@ -175,14 +175,20 @@ def _runs(case):
 
 
 class State:
-    """Inputs, outputs and handles of one case; its handles are closed with it."""
+    """Inputs, outputs and handles of one case."""
 
     def __init__(self, **fields):
         self.__dict__.update(fields)
 
+
+class _Open:
+    """A library handle, closed once neither its state nor a view of its memory is left."""
+
+    def __init__(self, handle):
+        self.handle = handle
+
     def __del__(self):
-        if self.__dict__.get("handle") is not None:
-            self.handle.close()
+        self.handle.close()
 
 
 def _gen(seed):
@@ -278,9 +284,10 @@ def _rope(shape, positions):
 
 
 class _Memory:
-    """A handle's device memory, for torch to see."""
+    """A handle's device memory, for torch to see; torch keeps this object as long as the view."""
 
-    def __init__(self, ptr, like):
+    def __init__(self, opened, ptr, like):
+        self.opened = opened
         self.__cuda_array_interface__ = {"data": (ptr, False), "shape": tuple(like.shape), "version": 2,
                                          "typestr": "<f2" if like.dtype == torch.float16 else "<f4"}
 
@@ -297,12 +304,12 @@ def _pages_in_library(case, chunks, calls, tables, k, v, bounds):
         kv.reserve(s, upto)
     if any(kv.pages(s).tolist() != t for s, t in tables.items()):
         raise RuntimeError("the sessions' pages are not the lowest free ones")
-    memory = kv.storage(0)
-    views = [torch.as_tensor(_Memory(ptr, x), device="cuda").copy_(x)
+    memory, opened = kv.storage(0), _Open(kv)
+    views = [torch.as_tensor(_Memory(opened, ptr, x), device="cuda").copy_(x)
              for ptr, x in zip((memory.keys, memory.values, memory.bounds), (k, v, bounds)) if x is not None]
     for s, start, _ in chunks:
         kv.set_length(0, int(s), int(start))  # the positions that the copied pages hold
-    return kv, views
+    return opened, views
 
 
 def prepare(case, seed):
@@ -321,7 +328,7 @@ def _prepare_pages(case, seed):
     state = State(kind=case["kind"], case=case, q=q, k=kn, v=vn, out=out, chosen=chosen)
     if own:
         A = _library()[0]
-        state.handle, state.pools = _pages_in_library(case, chunks, calls, tables, k, v, bounds)
+        state.opened, state.pools = _pages_in_library(case, chunks, calls, tables, k, v, bounds)
         state.layer = A.AttentionLayer(0, shape["heads"], case["window"], shape["neox"], rope=_rope(shape, length))
         state.chunks = chunks
         state.selection = A.PageSelection(case["top"], case["first"], case["last"]) if case["top"] else None
@@ -349,12 +356,13 @@ def _prepare_adapters(case, seed):
     if own:
         A, lib = _library()
         dtype = {"f16": A.ADAPTER_F16, "bf16": A.ADAPTER_BF16, "f32": A.ADAPTER_F32}[case["dtype"]]
-        state.handle = lib.adapters(case["slots"], case["cols"], case["outs"], int(rank.max()), dtype)
+        adapters = lib.adapters(case["slots"], case["cols"], case["outs"], int(rank.max()), dtype)
+        state.opened = _Open(adapters)
         for s in range(case["slots"]):
             n = int(rank[s])
             sa, sb = a[s, :n].contiguous(), b[s, :, :n].contiguous()
             torch.cuda.synchronize()
-            state.handle.load_device(s, n, sa.data_ptr(), sa.numel(), sb.data_ptr(), sb.numel(), float(scale[s]))
+            adapters.load_device(s, n, sa.data_ptr(), sa.numel(), sb.data_ptr(), sb.numel(), float(scale[s]))
             lib.synchronize()
         state.runs = runs
     else:
@@ -376,15 +384,15 @@ def _prepare_adapters(case, seed):
 def run(s):
     if s.kind == "adapters":
         if own:
-            s.handle.apply_device(s.runs, s.x.data_ptr(), s.x.numel(), s.base.data_ptr(), s.out.data_ptr(),
-                                  s.out.numel())
+            s.opened.handle.apply_device(s.runs, s.x.data_ptr(), s.x.numel(), s.base.data_ptr(),
+                                         s.out.data_ptr(), s.out.numel())
             return s.out
         return _plain_adapters(s)
     if own:
-        s.handle.forward_device(s.layer, s.chunks, s.q.data_ptr(), s.q.numel(), s.k.data_ptr(), s.k.numel(),
-                                s.v.data_ptr(), s.v.numel(), s.out.data_ptr(), s.out.numel(), s.selection,
-                                s.chosen.data_ptr() if s.chosen is not None else 0,
-                                s.chosen.numel() if s.chosen is not None else 0)
+        s.opened.handle.forward_device(s.layer, s.chunks, s.q.data_ptr(), s.q.numel(), s.k.data_ptr(), s.k.numel(),
+                                       s.v.data_ptr(), s.v.numel(), s.out.data_ptr(), s.out.numel(), s.selection,
+                                       s.chosen.data_ptr() if s.chosen is not None else 0,
+                                       s.chosen.numel() if s.chosen is not None else 0)
         return [s.out] + ([s.chosen] if s.chosen is not None else []) + s.pools
     return _plain_pages(s)
 
