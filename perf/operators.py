@@ -284,10 +284,9 @@ def _rope(shape, positions):
 
 
 class _Memory:
-    """A handle's device memory, for torch to see; torch keeps this object as long as the view."""
+    """A handle's device memory, for torch to see."""
 
-    def __init__(self, opened, ptr, like):
-        self.opened = opened
+    def __init__(self, ptr, like):
         self.__cuda_array_interface__ = {"data": (ptr, False), "shape": tuple(like.shape), "version": 2,
                                          "typestr": "<f2" if like.dtype == torch.float16 else "<f4"}
 
@@ -305,8 +304,10 @@ def _pages_in_library(case, chunks, calls, tables, k, v, bounds):
     if any(kv.pages(s).tolist() != t for s, t in tables.items()):
         raise RuntimeError("the sessions' pages are not the lowest free ones")
     memory, opened = kv.storage(0), _Open(kv)
-    views = [torch.as_tensor(_Memory(opened, ptr, x), device="cuda").copy_(x)
+    views = [torch.as_tensor(_Memory(ptr, x), device="cuda").copy_(x)
              for ptr, x in zip((memory.keys, memory.values, memory.bounds), (k, v, bounds)) if x is not None]
+    for view in views:
+        view.opened = opened  # returned as outputs, the views may be all that is left of the state
     for s, start, _ in chunks:
         kv.set_length(0, int(s), int(start))  # the positions that the copied pages hold
     return opened, views
