@@ -64,6 +64,10 @@ extern "C" {
                                             same call once outside the capture first (no
                                             counterpart in the reference, which has no graphs) */
 
+#define JMODELS_ATTN_OUT_OF_PAGES 10     /* a paged cache has too few free pages for the call: nothing was
+                                            changed (no counterpart in the reference, whose caches are
+                                            not paged) */
+
 /* Capability bits (RS:59-77 style). */
 #define JMODELS_ATTN_CAP_DECODE_F32 (1ull << 0)      /* f32 KV split-K decode */
 #define JMODELS_ATTN_CAP_DECODE_F16 (1ull << 1)      /* f16 KV split-K decode */
@@ -76,6 +80,9 @@ extern "C" {
 #define JMODELS_ATTN_CAP_VALUE_NORM (1ull << 8)      /* unweighted per-head RMS norm of v (Gemma 4) */
 #define JMODELS_ATTN_CAP_QUANT_MATMUL (1ull << 9)    /* Q4_0 / Q8_0 / Q5_0 / Q4_K / Q5_K / Q6_K
                                                         projections on device memory */
+#define JMODELS_ATTN_CAP_PAGED_KV (1ull << 10)       /* paged caches, chunks of many sequences in one call */
+#define JMODELS_ATTN_CAP_PAGE_SELECTION (1ull << 11) /* attention over pages chosen by their bounds */
+#define JMODELS_ATTN_CAP_ADAPTERS (1ull << 12)       /* low-rank adapters of many requests in one call */
 
 /* KV storage element types. F16 stores IEEE binary16 (round to nearest even), which widens to
  * exactly Float.float16ToFloat(Float.floatToFloat16(x)) — the reference's half-precision KV
@@ -399,6 +406,177 @@ JMODELS_ATTN_API int32_t jmodels_attn_quantized_grouped_matmul_device(
     const uint64_t* weight_bytes, const uint32_t* rows, uint32_t matrix_count, const float* input,
     uint64_t input_elements, float* output, uint64_t output_elements, uint32_t batch_size,
     uint32_t cols, const float* const* addends, uint32_t addend_mode);
+
+/* ---------------------------------------------------------------- paged KV cache
+ *
+ * Sequences that share a pool of pages instead of holding max_seq_len positions each (the reference's
+ * KvCache grows per session, BJ/cache/KvCache.java:284-322; it has no pages). A call takes chunks of
+ * new tokens of many sequences at once: prompts, parts of prompts and single tokens mixed. Every KV head
+ * count, query head count that is a multiple of it, head length 32, 64, 128 or 256 (keys and values
+ * alike) and layer parameter of the contiguous caches is taken; LINEAR retention only.
+ *
+ * A page holds page_slots (32, 64, 128 or 256) positions of every KV head in every layer. The library
+ * hands pages out, always the lowest-numbered free one. Position p of a sequence is slot
+ * p % page_slots of the page that is entry p / page_slots of its list. Storage of a layer (elements of
+ * the cache's type; W = 32 for f16, 16 for f32):
+ *   keys   [page][kv head][page_slots / 32][head_length / W][32][W]
+ *   values [page][kv head][page_slots / 32][head_length][32]
+ *   bounds [page][kv head][2][head_length]: smallest and largest key elements of the page's filled
+ *          slots after the last append to it (with JMODELS_ATTN_PAGED_BOUNDS)
+ *
+ * A sequence's positions are appended in order: a chunk starts at or before the layer's length, and
+ * the layer then ends with the chunk (what it held behind is given up; a speculative decode rewinds so).
+ * Appends take the pages they need; OUT_OF_PAGES changes nothing. A call that needs new pages cannot be
+ * captured (NOT_CAPTURABLE): reserve them before. A captured call reads the page lists as they are when
+ * it is replayed; its sequences, starts and row counts are those of the capture, and graphs that share a
+ * context are replayed one after another, on its stream. */
+typedef struct jmodels_attn_paged_kv jmodels_attn_paged_kv;
+
+/* `rows` new tokens of `sequence` at positions start .. start + rows - 1. The rows of a call's chunks lie
+ * one after another in q, k, v and out. A sequence appears once in a call; rows 0 is allowed. */
+typedef struct jmodels_attn_chunk {
+  uint32_t sequence;
+  uint32_t start;
+  uint32_t rows;
+} jmodels_attn_chunk;
+
+/* Which pages a token attends to: its sequence's first `first` pages, its last `last` ones (its own page
+ * is the last; last >= 1), and of the others the `top` that score highest; every page where there are no
+ * more than first + last + top. A page's score for a row and KV head is
+ *   max over the group's query heads of  sum_d max(q_d lo_d, q_d hi_d),
+ * which no key in the page exceeds, computed in 64 bits; of equal scores the lower page is taken, and
+ * a score that is no number counts as the highest. */
+typedef struct jmodels_attn_selection {
+  uint32_t top;
+  uint32_t first;
+  uint32_t last;
+} jmodels_attn_selection;
+
+#define JMODELS_ATTN_PAGED_BOUNDS 1u  /* keep page bounds: needed for selections */
+#define JMODELS_ATTN_NO_PAGE 0xFFFFFFFFu
+
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_create(jmodels_attn_context* ctx, uint32_t sequences,
+                                     uint32_t num_layers, uint32_t max_seq_len, uint32_t pages,
+                                     uint32_t page_slots, uint32_t num_kv_heads,
+                                     uint32_t head_length, uint32_t dtype, uint32_t flags,
+                                     jmodels_attn_paged_kv** kv_out);
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_destroy(jmodels_attn_paged_kv* kv);
+/* Pages for positions [0, length) of a sequence. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_reserve(jmodels_attn_paged_kv* kv, uint32_t sequence,
+                                      uint32_t length);
+/* KvCache.discardFrom (BJ/cache/KvCache.java:161-173): positions from `position` on are given up in
+ * every layer, and pages that hold nothing before it are free again, also reserved ones. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_discard_from(jmodels_attn_paged_kv* kv, uint32_t sequence,
+                                           uint32_t position);
+/* KvCache.clear (BJ/cache/KvCache.java:156-158) for one sequence, or all when sequence < 0. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_clear(jmodels_attn_paged_kv* kv, int32_t sequence);
+/* The target, a sequence without pages, gets the source's first `positions` (a multiple of page_slots,
+ * held in every layer) without copying them. Pages of several sequences are read-only: an append that
+ * would write to one is refused (UNAVAILABLE). */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_fork(jmodels_attn_paged_kv* kv, uint32_t source, uint32_t target,
+                                   uint32_t positions);
+/* Positions that a layer holds of a sequence. set_length declares them, for callers that write the
+ * storage themselves (a restored session, pages from another device), bounds included. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_length(const jmodels_attn_paged_kv* kv, uint32_t layer,
+                                     uint32_t sequence, uint32_t* length_out);
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_set_length(jmodels_attn_paged_kv* kv, uint32_t layer,
+                                         uint32_t sequence, uint32_t length);
+/* A sequence's list of pages (pages may be NULL: only its length is asked for). */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_pages(const jmodels_attn_paged_kv* kv, uint32_t sequence,
+                                    uint32_t* pages, uint64_t page_elements, uint32_t* count_out);
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_free_pages(const jmodels_attn_paged_kv* kv, uint32_t* count_out);
+/* Device addresses of a layer's keys, values and bounds (NULL without them), and the bytes of its keys
+ * (its values take as many). */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_storage(const jmodels_attn_paged_kv* kv, uint32_t layer,
+                                      void** keys_out, void** values_out, void** bounds_out,
+                                      uint64_t* bytes_out);
+/* Rows [from, to) in f32, as jmodels_attn_kv_read; either output may be NULL. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_kv_read(jmodels_attn_context* ctx, const jmodels_attn_paged_kv* kv,
+                                   uint32_t sequence, uint32_t layer, uint32_t from, uint32_t to,
+                                   float* keys, uint64_t key_elements, float* values,
+                                   uint64_t value_elements);
+
+/* The calls below take device pointers, 16-byte aligned, and are asynchronous on the context stream;
+ * out must not alias an input.
+ *
+ * append: QK-norm, RoPE and the store of every chunk's k and v; q_rotated (may be NULL: q is not read)
+ * gets the rotated queries. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_append_device(
+    jmodels_attn_context* ctx, jmodels_attn_paged_kv* kv, const jmodels_attn_layer* layer,
+    const jmodels_attn_chunk* chunks, uint32_t count, const float* q, uint64_t q_elements,
+    const float* k, uint64_t k_elements, const float* v, uint64_t v_elements, float* q_rotated,
+    uint64_t q_rotated_elements);
+/* select: the pages of every row of rotated queries, [rows][kv heads][first + last + top], ascending,
+ * JMODELS_ATTN_NO_PAGE behind the last. The rows are appended already. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_select_device(
+    jmodels_attn_context* ctx, const jmodels_attn_paged_kv* kv, const jmodels_attn_layer* layer,
+    const jmodels_attn_chunk* chunks, uint32_t count, const jmodels_attn_selection* selection,
+    const float* q, uint64_t q_elements, uint32_t* pages, uint64_t page_elements);
+/* attend: causal attention of rotated queries over every position [first, p] of their sequences, or
+ * (pages not NULL) over those in the listed pages, [rows][kv heads][budget], ascending,
+ * JMODELS_ATTN_NO_PAGE behind the last; a list that is not is reported by
+ * jmodels_attn_context_synchronize (OUT_OF_RANGE), its wrong entries left out. A sliding window
+ * cannot be combined with pages. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_attend_device(
+    jmodels_attn_context* ctx, const jmodels_attn_paged_kv* kv, const jmodels_attn_layer* layer,
+    const jmodels_attn_chunk* chunks, uint32_t count, const float* q, uint64_t q_elements,
+    float* out, uint64_t out_elements, const uint32_t* pages, uint64_t page_elements,
+    uint32_t budget);
+/* forward: append, select where `selection` is not NULL (pages, which may be NULL, gets the lists), and
+ * attend. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_forward_device(
+    jmodels_attn_context* ctx, jmodels_attn_paged_kv* kv, const jmodels_attn_layer* layer,
+    const jmodels_attn_chunk* chunks, uint32_t count, const float* q, uint64_t q_elements,
+    const float* k, uint64_t k_elements, const float* v, uint64_t v_elements, float* out,
+    uint64_t out_elements, const jmodels_attn_selection* selection, uint32_t* pages,
+    uint64_t page_elements);
+/* The same on host buffers, synchronous. */
+JMODELS_ATTN_API int32_t jmodels_attn_paged_forward(
+    jmodels_attn_context* ctx, jmodels_attn_paged_kv* kv, const jmodels_attn_layer* layer,
+    const jmodels_attn_chunk* chunks, uint32_t count, const float* q, uint64_t q_elements,
+    const float* k, uint64_t k_elements, const float* v, uint64_t v_elements, float* out,
+    uint64_t out_elements, const jmodels_attn_selection* selection, uint32_t* pages,
+    uint64_t page_elements);
+
+/* ---------------------------------------------------------------- low-rank adapters
+ *
+ * Beside a projection that many requests share, each request's own low-rank addition:
+ *   output[row] = base[row] + scale * B (A input[row])
+ * with A [rank][cols] and B [rows][rank] of the row's adapter. `slots` adapters of one projection are
+ * kept on the device in their stored type; sums are formed in f32. The reference has no adapters. */
+typedef struct jmodels_attn_adapters jmodels_attn_adapters;
+#define JMODELS_ATTN_ADAPTER_F32 0u
+#define JMODELS_ATTN_ADAPTER_F16 1u
+#define JMODELS_ATTN_ADAPTER_BF16 2u
+#define JMODELS_ATTN_NO_ADAPTER 0xFFFFFFFFu
+
+/* `rows` consecutive rows with the adapter in `slot`, or JMODELS_ATTN_NO_ADAPTER. */
+typedef struct jmodels_attn_adapter_run {
+  uint32_t slot;
+  uint32_t rows;
+} jmodels_attn_adapter_run;
+
+/* cols: a multiple of 8; rows: any; max_rank: 1 to 256. */
+JMODELS_ATTN_API int32_t jmodels_attn_adapters_create(jmodels_attn_context* ctx, uint32_t slots, uint32_t cols,
+                                     uint32_t rows, uint32_t max_rank, uint32_t dtype,
+                                     jmodels_attn_adapters** adapters_out);
+JMODELS_ATTN_API int32_t jmodels_attn_adapters_destroy(jmodels_attn_adapters* adapters);
+/* Copies an adapter's A and B (device pointers, the set's type) into a slot, on the context stream:
+ * calls made before keep the slot's old one. Not capturable. */
+JMODELS_ATTN_API int32_t jmodels_attn_adapters_load_device(jmodels_attn_adapters* adapters, uint32_t slot,
+                                          uint32_t rank, const void* a, uint64_t a_elements,
+                                          const void* b, uint64_t b_elements, float scale);
+JMODELS_ATTN_API int32_t jmodels_attn_adapters_unload(jmodels_attn_adapters* adapters, uint32_t slot);
+/* Runs of rows one after another, each with its adapter. input [rows][cols], base (NULL: zero) and
+ * output [rows][the set's rows] f32, device pointers, 16-byte aligned, asynchronous on the context
+ * stream. base may be output itself; input must not be. Rows without an adapter get base. A captured
+ * call keeps the ranks and scales of the capture and reads the weights at its replays. */
+JMODELS_ATTN_API int32_t jmodels_attn_adapters_apply_device(jmodels_attn_context* ctx,
+                                           const jmodels_attn_adapters* adapters,
+                                           const jmodels_attn_adapter_run* runs, uint32_t count,
+                                           const float* input, uint64_t input_elements,
+                                           const float* base, float* output,
+                                           uint64_t output_elements);
 
 #ifdef __cplusplus
 }

@@ -55,8 +55,11 @@ public final class HipAttentionLibrary implements AutoCloseable {
   public static final long CAP_QK_NORM = 1L << 7;
   public static final long CAP_VALUE_NORM = 1L << 8;
   public static final long CAP_QUANT_MATMUL = 1L << 9;
+  public static final long CAP_PAGED_KV = 1L << 10;
+  public static final long CAP_PAGE_SELECTION = 1L << 11;
+  public static final long CAP_ADAPTERS = 1L << 12;
 
-  // Status codes: 0-4 keep backend-native's meaning (RS:78-82), 5-9 are this library's.
+  // Status codes: 0-4 keep backend-native's meaning (RS:78-82), 5-10 are this library's.
   public static final int OK = 0;
   public static final int NULL_POINTER = 1;
   public static final int INVALID_SHAPE = 2;
@@ -67,6 +70,7 @@ public final class HipAttentionLibrary implements AutoCloseable {
   public static final int UNAVAILABLE = 7;
   public static final int NON_FINITE = 8;
   public static final int NOT_CAPTURABLE = 9;
+  public static final int OUT_OF_PAGES = 10;
 
   public static final int KV_F32 = 0;
   public static final int KV_F16 = 1;
@@ -74,6 +78,16 @@ public final class HipAttentionLibrary implements AutoCloseable {
   public static final int ADDEND_NONE = 0;
   public static final int ADDEND_BIAS = 1;
   public static final int ADDEND_RESIDUAL = 2;
+  public static final int PAGED_BOUNDS = 1;
+  public static final int ADAPTER_F32 = 0;
+  public static final int ADAPTER_F16 = 1;
+  public static final int ADAPTER_BF16 = 2;
+
+  /** A run of rows without an adapter (JMODELS_ATTN_NO_ADAPTER). */
+  public static final int NO_ADAPTER = 0xFFFFFFFF;
+
+  /** What stands behind the last page of a list (JMODELS_ATTN_NO_PAGE). */
+  public static final int NO_PAGE = 0xFFFFFFFF;
 
   /** jmodels_attn_layer: one layer's parameters for a call (40 bytes). */
   public static final StructLayout LAYER =
@@ -95,6 +109,20 @@ public final class HipAttentionLibrary implements AutoCloseable {
           JAVA_INT.withName("value_length"),
           JAVA_INT.withName("ring_capacity"));
 
+  /** jmodels_attn_chunk: new tokens of one sequence in a paged call (12 bytes). */
+  public static final StructLayout CHUNK =
+      MemoryLayout.structLayout(
+          JAVA_INT.withName("sequence"), JAVA_INT.withName("start"), JAVA_INT.withName("rows"));
+
+  /** jmodels_attn_selection: the pages a token attends to (12 bytes). */
+  public static final StructLayout SELECTION =
+      MemoryLayout.structLayout(
+          JAVA_INT.withName("top"), JAVA_INT.withName("first"), JAVA_INT.withName("last"));
+
+  /** jmodels_attn_adapter_run: rows that share an adapter (8 bytes). */
+  public static final StructLayout ADAPTER_RUN =
+      MemoryLayout.structLayout(JAVA_INT.withName("slot"), JAVA_INT.withName("rows"));
+
   // Parameter shapes shared by several entry points (uint32_t and int32_t are JAVA_INT, uint64_t
   // JAVA_LONG, float JAVA_FLOAT, every pointer ADDRESS).
   private static final FunctionDescriptor STATUS_OF_HANDLE = FunctionDescriptor.of(JAVA_INT, ADDRESS);
@@ -115,6 +143,11 @@ public final class HipAttentionLibrary implements AutoCloseable {
       FunctionDescriptor.of(
           JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT,
           ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG);
+
+  private static final FunctionDescriptor PAGED_FORWARD =
+      FunctionDescriptor.of(
+          JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG,
+          ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG, ADDRESS, ADDRESS, JAVA_LONG);
 
   /** Every export of include/jmodels_attn.h with its descriptor, in the header's order. */
   static final Map<String, FunctionDescriptor> DOWNCALLS =
@@ -174,7 +207,53 @@ public final class HipAttentionLibrary implements AutoCloseable {
           entry("jmodels_attn_quantized_grouped_matmul_device",
               FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS,
                   JAVA_INT, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG, JAVA_INT, JAVA_INT, ADDRESS,
-                  JAVA_INT)));
+                  JAVA_INT)),
+          entry("jmodels_attn_paged_kv_create",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
+                  JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS)),
+          entry("jmodels_attn_paged_kv_destroy", STATUS_OF_HANDLE),
+          entry("jmodels_attn_paged_kv_reserve",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT)),
+          entry("jmodels_attn_paged_kv_discard_from",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT)),
+          entry("jmodels_attn_paged_kv_clear", FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT)),
+          entry("jmodels_attn_paged_kv_fork",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT)),
+          entry("jmodels_attn_paged_kv_length",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS)),
+          entry("jmodels_attn_paged_kv_set_length",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT)),
+          entry("jmodels_attn_paged_kv_pages",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, ADDRESS, JAVA_LONG, ADDRESS)),
+          entry("jmodels_attn_paged_kv_free_pages",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS)),
+          entry("jmodels_attn_paged_kv_storage",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS)),
+          entry("jmodels_attn_paged_kv_read",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT,
+                  JAVA_INT, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG)),
+          entry("jmodels_attn_paged_append_device",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS,
+                  JAVA_LONG, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG)),
+          entry("jmodels_attn_paged_select_device",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS,
+                  ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG)),
+          entry("jmodels_attn_paged_attend_device",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS,
+                  JAVA_LONG, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG, JAVA_INT)),
+          entry("jmodels_attn_paged_forward_device", PAGED_FORWARD),
+          entry("jmodels_attn_paged_forward", PAGED_FORWARD),
+          entry("jmodels_attn_adapters_create",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
+                  JAVA_INT, ADDRESS)),
+          entry("jmodels_attn_adapters_destroy", STATUS_OF_HANDLE),
+          entry("jmodels_attn_adapters_load_device",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, JAVA_LONG, ADDRESS,
+                  JAVA_LONG, JAVA_FLOAT)),
+          entry("jmodels_attn_adapters_unload", FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT)),
+          entry("jmodels_attn_adapters_apply_device",
+              FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, JAVA_LONG,
+                  ADDRESS, ADDRESS, JAVA_LONG)));
 
   private final Arena arena;
   private final long capabilities;
@@ -622,6 +701,143 @@ public final class HipAttentionLibrary implements AutoCloseable {
           "quantized_matmul_device");
     } catch (Throwable t) {
       throw bridge("quantized_matmul_device", t);
+    }
+  }
+
+  // ---------------------------------------------------------------- paged cache
+
+  /** A cache of {@code pages} pages that {@code sequences} sequences share; see jmodels_attn.h. */
+  public synchronized MemorySegment pagedKvCreate(
+      int sequences, int numLayers, int maxSeqLen, int pages, int pageSlots, int numKvHeads,
+      int headLength, boolean halfPrecision, boolean bounds) {
+    ensureOpen();
+    try (Arena call = Arena.ofConfined()) {
+      MemorySegment result = out(call);
+      check((int) h("jmodels_attn_paged_kv_create")
+              .invokeExact(context, sequences, numLayers, maxSeqLen, pages, pageSlots, numKvHeads,
+                  headLength, halfPrecision ? KV_F16 : KV_F32, bounds ? PAGED_BOUNDS : 0, result),
+          "paged_kv_create");
+      return result.get(ADDRESS, 0);
+    } catch (Throwable t) {
+      throw bridge("paged_kv_create", t);
+    }
+  }
+
+  public synchronized void pagedKvDestroy(MemorySegment kv) {
+    destroy("jmodels_attn_paged_kv_destroy", kv);
+  }
+
+  /** Pages for positions [0, length) of a sequence. */
+  public synchronized void pagedKvReserve(MemorySegment kv, int sequence, int length) {
+    ensureOpen();
+    try {
+      check((int) h("jmodels_attn_paged_kv_reserve").invokeExact(kv, sequence, length), "paged_kv_reserve");
+    } catch (Throwable t) {
+      throw bridge("paged_kv_reserve", t);
+    }
+  }
+
+  public synchronized void pagedKvDiscardFrom(MemorySegment kv, int sequence, int position) {
+    ensureOpen();
+    try {
+      check((int) h("jmodels_attn_paged_kv_discard_from").invokeExact(kv, sequence, position),
+          "paged_kv_discard_from");
+    } catch (Throwable t) {
+      throw bridge("paged_kv_discard_from", t);
+    }
+  }
+
+  /** Shares the source's first positions (whole pages) with a sequence that has none. */
+  public synchronized void pagedKvFork(MemorySegment kv, int source, int target, int positions) {
+    ensureOpen();
+    try {
+      check((int) h("jmodels_attn_paged_kv_fork").invokeExact(kv, source, target, positions), "paged_kv_fork");
+    } catch (Throwable t) {
+      throw bridge("paged_kv_fork", t);
+    }
+  }
+
+  /**
+   * Chunks {sequence, start, rows} of new tokens on host buffers: append, and attention over every
+   * page, or over those that selection {top, first, last} (may be null) picks.
+   */
+  public synchronized void pagedForward(
+      MemorySegment kv, MemorySegment layer, int[][] chunks, float[] q, float[] k, float[] v,
+      int[] selection, float[] out) {
+    ensureOpen();
+    try (Arena call = Arena.ofConfined()) {
+      MemorySegment c = call.allocate(CHUNK, chunks.length);
+      for (int i = 0; i < chunks.length; i++) {
+        if (chunks[i].length != 3) throw new IllegalArgumentException("chunk " + i + " needs 3 values");
+        for (int j = 0; j < 3; j++) c.setAtIndex(JAVA_INT, 3L * i + j, chunks[i][j]);
+      }
+      if (selection != null && selection.length != 3) {
+        throw new IllegalArgumentException("a selection needs 3 values");
+      }
+      MemorySegment s = selection == null ? MemorySegment.NULL : call.allocateFrom(JAVA_INT, selection);
+      MemorySegment os = call.allocate(JAVA_FLOAT, out.length);
+      check((int) h("jmodels_attn_paged_forward")
+              .invokeExact(context, kv, layer, c, chunks.length, call.allocateFrom(JAVA_FLOAT, q),
+                  (long) q.length, call.allocateFrom(JAVA_FLOAT, k), (long) k.length,
+                  call.allocateFrom(JAVA_FLOAT, v), (long) v.length, os, (long) out.length, s,
+                  MemorySegment.NULL, 0L),
+          "paged_forward");
+      MemorySegment.copy(os, JAVA_FLOAT, 0, out, 0, out.length);
+    } catch (Throwable t) {
+      throw bridge("paged_forward", t);
+    }
+  }
+
+  // ---------------------------------------------------------------- low-rank adapters
+
+  public synchronized MemorySegment adaptersCreate(int slots, int cols, int rows, int maxRank, int dtype) {
+    ensureOpen();
+    try (Arena call = Arena.ofConfined()) {
+      MemorySegment result = out(call);
+      check((int) h("jmodels_attn_adapters_create")
+              .invokeExact(context, slots, cols, rows, maxRank, dtype, result),
+          "adapters_create");
+      return result.get(ADDRESS, 0);
+    } catch (Throwable t) {
+      throw bridge("adapters_create", t);
+    }
+  }
+
+  public synchronized void adaptersDestroy(MemorySegment adapters) {
+    destroy("jmodels_attn_adapters_destroy", adapters);
+  }
+
+  /** A [rank][cols] and B [rows][rank] on device memory into a slot. */
+  public synchronized void adaptersLoadDevice(
+      MemorySegment adapters, int slot, int rank, MemorySegment a, long aElements, MemorySegment b,
+      long bElements, float scale) {
+    ensureOpen();
+    try {
+      check((int) h("jmodels_attn_adapters_load_device")
+              .invokeExact(adapters, slot, rank, a, aElements, b, bElements, scale),
+          "adapters_load_device");
+    } catch (Throwable t) {
+      throw bridge("adapters_load_device", t);
+    }
+  }
+
+  /** Runs {slot or NO_ADAPTER, rows} of one projection's rows, on device memory. */
+  public synchronized void adaptersApplyDevice(
+      MemorySegment adapters, int[][] runs, MemorySegment input, long inputElements,
+      MemorySegment base, MemorySegment output, long outputElements) {
+    ensureOpen();
+    try (Arena call = Arena.ofConfined()) {
+      MemorySegment r = call.allocate(ADAPTER_RUN, runs.length);
+      for (int i = 0; i < runs.length; i++) {
+        if (runs[i].length != 2) throw new IllegalArgumentException("run " + i + " needs 2 values");
+        for (int j = 0; j < 2; j++) r.setAtIndex(JAVA_INT, 2L * i + j, runs[i][j]);
+      }
+      check((int) h("jmodels_attn_adapters_apply_device")
+              .invokeExact(context, adapters, r, runs.length, input, inputElements,
+                  base == null ? MemorySegment.NULL : base, output, outputElements),
+          "adapters_apply_device");
+    } catch (Throwable t) {
+      throw bridge("adapters_apply_device", t);
     }
   }
 

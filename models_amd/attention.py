@@ -10,6 +10,9 @@ This is the host side above the C ABI (``include/jmodels_attn.h``). Names follow
 * :class:`HipKvCache` — ``cache/KvCache.java`` / ``cache/LayeredKvCache.java`` resident in HBM:
   ``store``, ``key_slice``/``value_slice``, ``contains``, ``discard_from``, ``clear``.
 * :class:`HipQkNorm` — a layer's QK-norm weights (``LlamaForwardPass.normalizeHead``).
+* :class:`HipPagedKvCache` — sequences that share a pool of pages; chunks of many sequences in one
+  call, and attention over the pages that :class:`PageSelection` picks.
+* :class:`HipAdapters` — low-rank adapters of many requests beside a shared projection.
 * :class:`AttentionLayer` — the per-layer flags ``LlamaConfig`` supplies (heads, window, NeoX,
   scale, RoPE table, QK-norm).
 * ``decode`` / ``attend`` / ``append`` / ``prefill`` — the attention block of
@@ -43,6 +46,7 @@ OUT_OF_RANGE = 6
 UNAVAILABLE = 7
 NON_FINITE = 8
 NOT_CAPTURABLE = 9
+OUT_OF_PAGES = 10
 
 CAP_DECODE_F32 = 1 << 0
 CAP_DECODE_F16 = 1 << 1
@@ -53,6 +57,10 @@ CAP_RING_LAYERS = 1 << 5
 CAP_DEVICE_POINTERS = 1 << 6
 CAP_QK_NORM = 1 << 7
 CAP_VALUE_NORM = 1 << 8
+CAP_QUANT_MATMUL = 1 << 9
+CAP_PAGED_KV = 1 << 10
+CAP_PAGE_SELECTION = 1 << 11
+CAP_ADAPTERS = 1 << 12
 
 NORM_VALUE_RMS = 1
 
@@ -67,6 +75,12 @@ WEIGHTS_Q5_0 = 5
 ADDEND_NONE = 0
 ADDEND_BIAS = 1
 ADDEND_RESIDUAL = 2
+PAGED_BOUNDS = 1
+NO_PAGE = 0xFFFFFFFF
+ADAPTER_F32 = 0
+ADAPTER_F16 = 1
+ADAPTER_BF16 = 2
+NO_ADAPTER = 0xFFFFFFFF
 
 EXPORTS = (
     "jmodels_attn_abi_version", "jmodels_attn_capabilities", "jmodels_attn_status_name",
@@ -81,7 +95,16 @@ EXPORTS = (
     "jmodels_attn_attend_causal_device", "jmodels_attn_norm_create", "jmodels_attn_norm_create_ex",
     "jmodels_attn_norm_destroy", "jmodels_attn_decode_device_noalloc",
     "jmodels_attn_kv_create_layered", "jmodels_attn_quantized_matmul_device",
-    "jmodels_attn_quantized_grouped_matmul_device",
+    "jmodels_attn_quantized_grouped_matmul_device", "jmodels_attn_paged_kv_create",
+    "jmodels_attn_paged_kv_destroy", "jmodels_attn_paged_kv_reserve",
+    "jmodels_attn_paged_kv_discard_from", "jmodels_attn_paged_kv_clear", "jmodels_attn_paged_kv_fork",
+    "jmodels_attn_paged_kv_length", "jmodels_attn_paged_kv_set_length", "jmodels_attn_paged_kv_pages",
+    "jmodels_attn_paged_kv_free_pages", "jmodels_attn_paged_kv_storage", "jmodels_attn_paged_kv_read",
+    "jmodels_attn_paged_append_device", "jmodels_attn_paged_select_device",
+    "jmodels_attn_paged_attend_device", "jmodels_attn_paged_forward_device",
+    "jmodels_attn_paged_forward", "jmodels_attn_adapters_create", "jmodels_attn_adapters_destroy",
+    "jmodels_attn_adapters_load_device", "jmodels_attn_adapters_unload",
+    "jmodels_attn_adapters_apply_device",
 )
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -150,6 +173,25 @@ def _declare(lib: ctypes.CDLL) -> None:
         "jmodels_attn_kv_read": (_i32, [_vp, _vp, _u32, _u32, _u32, _u32, _vp, _u64, _vp, _u64]),
         "jmodels_attn_kv_bytes": (_i32, [_vp, ctypes.POINTER(_u64)]),
     }
+    for name, tail in {
+            "create": [_u32] * 9 + [ctypes.POINTER(_vp)], "destroy": [], "reserve": [_u32, _u32],
+            "discard_from": [_u32, _u32], "clear": [_i32], "fork": [_u32, _u32, _u32],
+            "length": [_u32, _u32, _vp], "set_length": [_u32, _u32, _u32],
+            "pages": [_u32, _vp, _u64, _vp], "free_pages": [_vp],
+            "storage": [_u32, _vp, _vp, _vp, _vp],
+            "read": [_vp, _u32, _u32, _u32, _u32, _vp, _u64, _vp, _u64]}.items():
+        sig["jmodels_attn_paged_kv_" + name] = (_i32, [_vp] + tail)
+    chunked = [_vp, _vp, _LP, _vp, _u32]
+    sig["jmodels_attn_paged_append_device"] = (_i32, chunked + [_vp, _u64] * 4)
+    sig["jmodels_attn_paged_select_device"] = (_i32, chunked + [_vp, _vp, _u64, _vp, _u64])
+    sig["jmodels_attn_paged_attend_device"] = (_i32, chunked + [_vp, _u64] * 3 + [_u32])
+    for name in ("jmodels_attn_paged_forward_device", "jmodels_attn_paged_forward"):
+        sig[name] = (_i32, chunked + [_vp, _u64] * 4 + [_vp, _vp, _u64])
+    sig["jmodels_attn_adapters_create"] = (_i32, [_vp, _u32, _u32, _u32, _u32, _u32, ctypes.POINTER(_vp)])
+    sig["jmodels_attn_adapters_destroy"] = (_i32, [_vp])
+    sig["jmodels_attn_adapters_load_device"] = (_i32, [_vp, _u32, _u32, _vp, _u64, _vp, _u64, _cf])
+    sig["jmodels_attn_adapters_unload"] = (_i32, [_vp, _u32])
+    sig["jmodels_attn_adapters_apply_device"] = (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _vp, _vp, _u64])
     rows = [_vp, _vp, _LP, _u32, _u32p, _u32p]
     for name in ("jmodels_attn_append", "jmodels_attn_append_device"):
         sig[name] = (_i32, rows + [_vp, _u64, _vp, _u64, _vp, _u64, _vp, _u64])
@@ -302,6 +344,18 @@ class HipAttentionLibrary:
         (gemma4/Gemma4KvCache.java:39-47)."""
         return HipKvCache(self, list(specs), max_seq_len, half_precision, sequences, uniform=False)
 
+    def paged_kv_cache(self, num_layers: int, max_seq_len: int, pages: int, page_slots: int,
+                       num_kv_heads: int, head_length: int, half_precision: bool = True,
+                       sequences: int = 1, page_bounds: bool = False) -> "HipPagedKvCache":
+        """Sequences of up to max_seq_len positions that share `pages` pages of page_slots positions
+        each; page_bounds: keep what selections score pages by."""
+        return HipPagedKvCache(self, num_layers, max_seq_len, pages, page_slots, num_kv_heads,
+                               head_length, half_precision, sequences, page_bounds)
+
+    def adapters(self, slots: int, cols: int, rows: int, max_rank: int,
+                 dtype: int = ADAPTER_F16) -> "HipAdapters":
+        """Low-rank adapters of one projection of `cols` inputs and `rows` outputs."""
+        return HipAdapters(self, slots, cols, rows, max_rank, dtype)
 
     # ---- quantized projections (device pointers, asynchronous on the context stream)
 
@@ -693,6 +747,226 @@ class HipKvCache:
         o.check(o.lib.jmodels_attn_prefill_device(
             o.ctx, self.handle, ctypes.byref(st), sequence, start, n, q_ptr, q_elems, k_ptr,
             k_elems, v_ptr, v_elems, out_ptr, out_elems), "prefill_device")
+
+
+@dataclass(frozen=True)
+class PageSelection:
+    """The pages a token attends to: its sequence's `first` first and `last` last ones, and the `top`
+    others whose bounds promise the largest scores."""
+
+    top: int
+    first: int = 1
+    last: int = 1
+
+    @property
+    def budget(self) -> int:
+        return self.top + self.first + self.last
+
+    def struct(self):
+        return (_u32 * 3)(self.top, self.first, self.last)
+
+
+@dataclass(frozen=True)
+class PagedStorage:
+    """Device addresses of a layer's keys, values and bounds (None without them), and the bytes of its
+    keys (its values take as many); the layouts stand in include/jmodels_attn.h."""
+
+    keys: int
+    values: int
+    bounds: Optional[int]
+    bytes: int
+
+
+def _list2(a, width: int, what: str) -> np.ndarray:
+    x = np.ascontiguousarray(a)
+    if x.ndim != 2 or x.shape[1] != width or x.shape[0] == 0:
+        raise ValueError(f"{what} must be a non-empty list of {width} numbers each")
+    if x.dtype != np.uint32:
+        y = x.astype(np.uint32)
+        if x.dtype.kind not in "iu" or (y != x).any():
+            raise ValueError(f"{what} must be whole numbers of 32 bits")
+        x = y
+    return x
+
+
+class HipPagedKvCache:
+    """Device-resident KV cache of pages that sequences share. Calls take chunks: rows of
+    (sequence, first position, new rows), whose rows lie one after another in q, k, v and out."""
+
+    def __init__(self, owner: HipAttentionLibrary, num_layers: int, max_seq_len: int, pages: int,
+                 page_slots: int, num_kv_heads: int, head_length: int, half_precision: bool,
+                 sequences: int, page_bounds: bool):
+        self.owner = owner
+        self.num_layers, self.max_seq_len, self.page_slots = num_layers, max_seq_len, page_slots
+        self.num_kv_heads, self.head_length = num_kv_heads, head_length
+        self.half_precision, self.sequences, self.page_bounds = half_precision, sequences, page_bounds
+        out = _vp()
+        owner.check(owner.lib.jmodels_attn_paged_kv_create(
+            owner.ctx, sequences, num_layers, max_seq_len, pages, page_slots, num_kv_heads, head_length,
+            KV_F16 if half_precision else KV_F32, PAGED_BOUNDS if page_bounds else 0, ctypes.byref(out)),
+            "paged_kv_create")
+        self.handle = out.value
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            self.owner.check(self.owner.lib.jmodels_attn_paged_kv_destroy(self.handle), "paged_kv_destroy")
+            self.handle = None
+
+    # ---- pages
+
+    def reserve(self, sequence: int, length: int) -> None:
+        """Pages for the sequence's positions [0, length)."""
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_reserve(self.handle, sequence, length), "paged_kv_reserve")
+
+    def discard_from(self, position: int, sequence: int = 0) -> None:
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_discard_from(self.handle, sequence, position),
+                "paged_kv_discard_from")
+
+    def clear(self, sequence: int = -1) -> None:
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_clear(self.handle, sequence), "paged_kv_clear")
+
+    def fork(self, source: int, target: int, positions: int) -> None:
+        """The target sequence gets the source's first positions (whole pages), shared."""
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_fork(self.handle, source, target, positions), "paged_kv_fork")
+
+    def length(self, layer: int, sequence: int = 0) -> int:
+        out = _u32()
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_length(self.handle, layer, sequence, ctypes.byref(out)),
+                "paged_kv_length")
+        return out.value
+
+    def set_length(self, layer: int, sequence: int, length: int) -> None:
+        """Declares positions whose storage the caller wrote."""
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_set_length(self.handle, layer, sequence, length),
+                "paged_kv_set_length")
+
+    def pages(self, sequence: int = 0) -> np.ndarray:
+        """The sequence's page numbers, in order."""
+        n = _u32()
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_pages(self.handle, sequence, None, 0, ctypes.byref(n)),
+                "paged_kv_pages")
+        out = np.empty(n.value, np.uint32)
+        o.check(o.lib.jmodels_attn_paged_kv_pages(self.handle, sequence, out.ctypes.data, out.size,
+                                                  ctypes.byref(n)), "paged_kv_pages")
+        return out
+
+    def free_pages(self) -> int:
+        out = _u32()
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_free_pages(self.handle, ctypes.byref(out)), "paged_kv_free_pages")
+        return out.value
+
+    def storage(self, layer: int) -> PagedStorage:
+        k, v, b, n = _vp(), _vp(), _vp(), _u64()
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_storage(self.handle, layer, ctypes.byref(k), ctypes.byref(v),
+                                                    ctypes.byref(b), ctypes.byref(n)), "paged_kv_storage")
+        return PagedStorage(k.value, v.value, b.value, n.value)
+
+    def read(self, layer: int, frm: int, to: int, sequence: int = 0):
+        n = max(to - frm, 0) * self.num_kv_heads * self.head_length
+        keys, values = np.empty(n, np.float32), np.empty(n, np.float32)
+        o = self.owner
+        o.check(o.lib.jmodels_attn_paged_kv_read(o.ctx, self.handle, sequence, layer, frm, to, _ptr(keys), n,
+                                                 _ptr(values), n), "paged_kv_read")
+        return keys, values
+
+    # ---- device pointers, asynchronous on the context stream
+
+    def append_device(self, layer: AttentionLayer, chunks, q_ptr: int, q_elems: int, k_ptr: int,
+                      k_elems: int, v_ptr: int, v_elems: int, qrot_ptr: int = 0,
+                      qrot_elems: int = 0) -> None:
+        """QK-norm, RoPE and the store of the chunks' rows; the rotated queries where asked for."""
+        c, st, o = _list2(chunks, 3, "chunks"), layer.struct(), self.owner
+        o.check(o.lib.jmodels_attn_paged_append_device(
+            o.ctx, self.handle, ctypes.byref(st), _ptr(c), len(c), q_ptr or None, q_elems, k_ptr, k_elems,
+            v_ptr, v_elems, qrot_ptr or None, qrot_elems), "paged_append_device")
+
+    def select_device(self, layer: AttentionLayer, chunks, selection: PageSelection, q_ptr: int,
+                      q_elems: int, pages_ptr: int, page_elems: int) -> None:
+        """The pages of every row of rotated queries: uint32 [rows][kv heads][selection.budget]."""
+        c, st, sel, o = _list2(chunks, 3, "chunks"), layer.struct(), selection.struct(), self.owner
+        o.check(o.lib.jmodels_attn_paged_select_device(
+            o.ctx, self.handle, ctypes.byref(st), _ptr(c), len(c), sel, q_ptr, q_elems, pages_ptr,
+            page_elems), "paged_select_device")
+
+    def attend_device(self, layer: AttentionLayer, chunks, q_ptr: int, q_elems: int, out_ptr: int,
+                      out_elems: int, pages_ptr: int = 0, page_elems: int = 0, budget: int = 0) -> None:
+        """Causal attention of rotated queries, over every page or the listed ones."""
+        c, st, o = _list2(chunks, 3, "chunks"), layer.struct(), self.owner
+        o.check(o.lib.jmodels_attn_paged_attend_device(
+            o.ctx, self.handle, ctypes.byref(st), _ptr(c), len(c), q_ptr, q_elems, out_ptr, out_elems,
+            pages_ptr or None, page_elems, budget), "paged_attend_device")
+
+    def forward_device(self, layer: AttentionLayer, chunks, q_ptr: int, q_elems: int, k_ptr: int,
+                       k_elems: int, v_ptr: int, v_elems: int, out_ptr: int, out_elems: int,
+                       selection: Optional[PageSelection] = None, pages_ptr: int = 0,
+                       page_elems: int = 0) -> None:
+        """Append, select where a selection is given, and attend."""
+        c, st, o = _list2(chunks, 3, "chunks"), layer.struct(), self.owner
+        o.check(o.lib.jmodels_attn_paged_forward_device(
+            o.ctx, self.handle, ctypes.byref(st), _ptr(c), len(c), q_ptr, q_elems, k_ptr, k_elems, v_ptr,
+            v_elems, out_ptr, out_elems, selection.struct() if selection is not None else None,
+            pages_ptr or None, page_elems), "paged_forward_device")
+
+    # ---- host buffers, synchronous
+
+    def forward(self, layer: AttentionLayer, chunks, q, k, v, selection: Optional[PageSelection] = None):
+        """forward_device on host buffers; returns out, and the selected pages with a selection."""
+        c, st, o = _list2(chunks, 3, "chunks"), layer.struct(), self.owner
+        q, k, v = _f32(q), _f32(k), _f32(v)
+        rows = int(c[:, 2].sum())
+        out = np.empty(rows * layer.num_heads * self.head_length, np.float32)
+        pages = np.empty((rows, self.num_kv_heads, selection.budget), np.uint32) if selection else None
+        o.check(o.lib.jmodels_attn_paged_forward(
+            o.ctx, self.handle, ctypes.byref(st), _ptr(c), len(c), _ptr(q), q.size, _ptr(k), k.size,
+            _ptr(v), v.size, _ptr(out), out.size, selection.struct() if selection else None,
+            _ptr(pages) if selection else None, pages.size if selection else 0), "paged_forward")
+        return (out, pages) if selection else out
+
+
+class HipAdapters:
+    """Low-rank adapters of one projection: output = base + scale * B (A input), each run of rows with
+    the adapter in its slot."""
+
+    def __init__(self, owner: HipAttentionLibrary, slots: int, cols: int, rows: int, max_rank: int, dtype: int):
+        self.owner = owner
+        self.slots, self.cols, self.rows, self.max_rank, self.dtype = slots, cols, rows, max_rank, dtype
+        out = _vp()
+        owner.check(owner.lib.jmodels_attn_adapters_create(owner.ctx, slots, cols, rows, max_rank, dtype,
+                                                           ctypes.byref(out)), "adapters_create")
+        self.handle = out.value
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            self.owner.check(self.owner.lib.jmodels_attn_adapters_destroy(self.handle), "adapters_destroy")
+            self.handle = None
+
+    def load_device(self, slot: int, rank: int, a_ptr: int, a_elems: int, b_ptr: int, b_elems: int,
+                    scale: float = 1.0) -> None:
+        """A [rank][cols] and B [rows][rank] of the set's type into a slot."""
+        o = self.owner
+        o.check(o.lib.jmodels_attn_adapters_load_device(self.handle, slot, rank, a_ptr, a_elems, b_ptr,
+                                                        b_elems, scale), "adapters_load_device")
+
+    def unload(self, slot: int) -> None:
+        o = self.owner
+        o.check(o.lib.jmodels_attn_adapters_unload(self.handle, slot), "adapters_unload")
+
+    def apply_device(self, runs, x_ptr: int, x_elems: int, base_ptr: int, out_ptr: int,
+                     out_elems: int) -> None:
+        """runs: rows of (slot or NO_ADAPTER, rows); base 0: the additions alone."""
+        r, o = _list2(runs, 2, "runs"), self.owner
+        o.check(o.lib.jmodels_attn_adapters_apply_device(o.ctx, self.handle, _ptr(r), len(r), x_ptr, x_elems,
+                                                         base_ptr or None, out_ptr, out_elems),
+                "adapters_apply_device")
 
 
 def default_scale(key_length: int) -> float:

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "jma_adapters.h"
+#include "jma_paged.h"
 #include "jma_plan.h"
 
 namespace jma {
@@ -323,5 +325,20 @@ hipError_t launch_q8_k_quant(const float* x, uint32_t batch, uint32_t cols, void
                              void* sums, void* scales, hipStream_t stream);
 hipError_t launch_qkgemm(const QMatArgs& a, uint32_t fmt, uint32_t shape, uint32_t tiles_w,
                          const void* act, const void* sums, const void* scales, hipStream_t stream);
+
+// ---------------------------------------------------------------- paged cache (jma_paged.hip)
+
+// RoPE, norms and the store of the chunks' rows (a.num_heads 0 with no q_out), then the bounds of the
+// pages written where the cache keeps them.
+hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, hipStream_t stream);
+// max_pages: pages that the row furthest back sees.
+hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, uint32_t max_pages, hipStream_t stream);
+hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, hipStream_t stream);
+hipError_t launch_paged_table(const PagedTableArgs& a, hipStream_t stream);
+
+// ---------------------------------------------------------------- low-rank adapters (jma_adapters.hip)
+
+hipError_t launch_adapter_load(const AdapterLoadArgs& a, hipStream_t stream);
+hipError_t launch_adapter_apply(const AdapterArgs& a, hipStream_t stream);
 
 }  // namespace jma

@@ -170,6 +170,9 @@ struct jmodels_attn_context {
   DeviceBuffer part_acc, part_ml, part_f, counters, pf_part, pf_tickets, qrot, stage_q, stage_k, stage_v, stage_out;
   DeviceBuffer qact;                // quantized activations of prefill-sized projections
   DeviceBuffer pp_part, pp_tickets; // split stripe pairs of the head-dim-512 f16 prefill
+  // paged cache: split states and their tickets, rotated queries, page scores, selected pages
+  DeviceBuffer paged_part, paged_tickets, paged_qrot, paged_keys, paged_select_tickets, paged_lists;
+  DeviceBuffer adapter_down;        // A x of low-rank adapters
   int decode_target_blocks = 512;   // workgroups a decode launch aims for (two per CU)
   int tiles_per_wave = 1;           // minimum tiles each decode wave streams
   int min_split_tiles = 0;          // minimum tiles per decode split; 0: waves x tiles_per_wave
@@ -287,15 +290,14 @@ struct LayerCall {
   const jmodels_attn_norm* norm;  // null or weights on neither side = no QK-norm
 };
 
-LayerCall resolve_layer(const jmodels_attn_kv* kv, const jmodels_attn_layer* p) {
-  require(p != nullptr, JMODELS_ATTN_NULL_POINTER, "layer parameters are null");
-  require(p->layer < kv->layers, JMODELS_ATTN_OUT_OF_RANGE,
-          "layer out of range: " + std::to_string(p->layer));
+// The parameters of a layer of hkv kv heads and key and value lengths dk and dv, in a cache of `ctx`.
+LayerCall layer_call(const jmodels_attn_context* ctx, const jmodels_attn_layer* p, uint32_t hkv, uint32_t dk,
+                     uint32_t dv) {
   LayerCall c{};
   c.layer = p->layer;
-  c.hkv = kv->hkv_l[p->layer];
-  c.dk = kv->dk_l[p->layer];
-  c.dv = kv->dv_l[p->layer];
+  c.hkv = hkv;
+  c.dk = dk;
+  c.dv = dv;
   require(p->num_heads > 0 && p->num_heads % c.hkv == 0, JMODELS_ATTN_INVALID_SHAPE,
           "num_heads must be a positive multiple of the layer's num_kv_heads");
   c.num_heads = p->num_heads;
@@ -307,12 +309,12 @@ LayerCall resolve_layer(const jmodels_attn_kv* kv, const jmodels_attn_layer* p) 
   require(isfinite(c.scale) && c.scale > 0.0f, JMODELS_ATTN_INVALID_SHAPE, "scale must be finite and > 0");
   c.rope = p->rope;
   if (c.rope) {
-    require(c.rope->ctx == kv->ctx, JMODELS_ATTN_INVALID_SHAPE, "rope table belongs to another context");
+    require(c.rope->ctx == ctx, JMODELS_ATTN_INVALID_SHAPE, "rope table belongs to another context");
     require(c.rope->rotary_dim <= c.dk, JMODELS_ATTN_INVALID_SHAPE, "rotary_dim exceeds key_length");
   }
   c.norm = p->qk_norm;
   if (c.norm) {
-    require(c.norm->ctx == kv->ctx, JMODELS_ATTN_INVALID_SHAPE, "qk-norm belongs to another context");
+    require(c.norm->ctx == ctx, JMODELS_ATTN_INVALID_SHAPE, "qk-norm belongs to another context");
     require(c.norm->head_dim == c.dk, JMODELS_ATTN_INVALID_SHAPE,
             "qk-norm head_dim differs from key_length");
     require(!c.norm->v_rms || c.norm->head_dim == c.dv, JMODELS_ATTN_INVALID_SHAPE,
@@ -320,6 +322,13 @@ LayerCall resolve_layer(const jmodels_attn_kv* kv, const jmodels_attn_layer* p) 
     if (!c.norm->d_q && !c.norm->d_k && !c.norm->v_rms) c.norm = nullptr;
   }
   return c;
+}
+
+LayerCall resolve_layer(const jmodels_attn_kv* kv, const jmodels_attn_layer* p) {
+  require(p != nullptr, JMODELS_ATTN_NULL_POINTER, "layer parameters are null");
+  require(p->layer < kv->layers, JMODELS_ATTN_OUT_OF_RANGE,
+          "layer out of range: " + std::to_string(p->layer));
+  return layer_call(kv->ctx, p, kv->hkv_l[p->layer], kv->dk_l[p->layer], kv->dv_l[p->layer]);
 }
 
 void check_rows(const jmodels_attn_kv* kv, const LayerCall& lc, uint32_t count,
@@ -793,6 +802,8 @@ void raise_errors(jmodels_attn_context* ctx) {
       hip_check(jma::fixed_scratch_reset(ctx->fixed, ctx->stream), "reset fixed scratch");
       fail(JMODELS_ATTN_DEVICE_ERROR, "cross-split reduction timed out waiting for a partial");
     }
+    if (err & 0xFF0000)
+      fail(JMODELS_ATTN_OUT_OF_RANGE, "a list of selected pages names a page past its row's position, or is not ascending");
     fail(JMODELS_ATTN_NON_FINITE, "softmax input contains NaN or positive infinity");
   }
 }
@@ -1024,7 +1035,8 @@ uint64_t jmodels_attn_capabilities(void) {
   return JMODELS_ATTN_CAP_DECODE_F32 | JMODELS_ATTN_CAP_DECODE_F16 | JMODELS_ATTN_CAP_PREFILL_MFMA |
          JMODELS_ATTN_CAP_RAGGED_DECODE | JMODELS_ATTN_CAP_SLIDING_WINDOW |
          JMODELS_ATTN_CAP_RING_LAYERS | JMODELS_ATTN_CAP_DEVICE_POINTERS | JMODELS_ATTN_CAP_QK_NORM |
-         JMODELS_ATTN_CAP_VALUE_NORM | JMODELS_ATTN_CAP_QUANT_MATMUL;
+         JMODELS_ATTN_CAP_VALUE_NORM | JMODELS_ATTN_CAP_QUANT_MATMUL | JMODELS_ATTN_CAP_PAGED_KV |
+         JMODELS_ATTN_CAP_PAGE_SELECTION | JMODELS_ATTN_CAP_ADAPTERS;
 }
 
 const char* jmodels_attn_status_name(int32_t status) {
@@ -1039,6 +1051,7 @@ const char* jmodels_attn_status_name(int32_t status) {
     case JMODELS_ATTN_UNAVAILABLE: return "UNAVAILABLE";
     case JMODELS_ATTN_NON_FINITE: return "NON_FINITE";
     case JMODELS_ATTN_NOT_CAPTURABLE: return "NOT_CAPTURABLE";
+    case JMODELS_ATTN_OUT_OF_PAGES: return "OUT_OF_PAGES";
     default: return "UNKNOWN";
   }
 }
@@ -1090,7 +1103,8 @@ int32_t jmodels_attn_context_destroy(jmodels_attn_context* ctx) {
     (void)hipStreamSynchronize(ctx->stream);
     for (DeviceBuffer* b : {&ctx->part_acc, &ctx->part_ml, &ctx->part_f, &ctx->counters, &ctx->pf_part, &ctx->pf_tickets, &ctx->qrot, &ctx->stage_q,
                             &ctx->stage_k, &ctx->stage_v, &ctx->stage_out, &ctx->qact, &ctx->pp_part,
-                            &ctx->pp_tickets})
+                            &ctx->pp_tickets, &ctx->paged_part, &ctx->paged_tickets, &ctx->paged_qrot,
+                            &ctx->paged_keys, &ctx->paged_select_tickets, &ctx->paged_lists, &ctx->adapter_down})
       b->release();
     (void)hipHostFree(ctx->host);
     (void)hipStreamDestroy(ctx->stream);
@@ -1903,3 +1917,7 @@ int32_t jmodels_attn_quantized_grouped_matmul_device(
 }
 
 }  // extern "C"
+
+// The host simulation of the tests builds the runtime from this one file.
+#include "jma_runtime_paged.inc"
+#include "jma_runtime_adapters.inc"

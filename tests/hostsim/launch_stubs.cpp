@@ -10,6 +10,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <functional>
 #include <string>
 #include <vector>
 
@@ -256,6 +257,159 @@ hipError_t launch_qkgemm(const QMatArgs& a, uint32_t fmt, uint32_t, uint32_t, co
   if (fmt != 3) add(l, sums, rows * (a.cols / 16) * 2, "activation sums");
   add(l, scales, rows * a.blocks * 4, "activation scales");
   return submit(stream, "qkgemm_kernel", l);
+}
+
+// ---------------------------------------------------------------- paged cache and adapters
+//
+// What these kernels touch depends on the page tables, which the simulated table launches write: the
+// checks read them when the launch executes, as the kernels do.
+
+namespace {
+
+hipError_t run(hipStream_t stream, const char* kernel, std::function<void()> f) {
+  auto* fn = new std::function<void()>(std::move(f));
+  return hipsim_launch(stream, kernel, [](void* p) { (*(std::function<void()>*)p)(); }, fn,
+                       [](void* p) { delete (std::function<void()>*)p; });
+}
+
+void check(const void* p, uint64_t bytes, const char* what) {
+  if (bytes) hipsim_check_range(p, bytes, what);
+}
+
+// Pages [from, to] of a sequence's list: in the pool, their K, V and bounds of every kv head.
+void check_pages(const PagedView& kv, uint32_t seq, uint32_t from, uint32_t to, uint32_t d, size_t es) {
+  const uint32_t* t = kv.table + (uint64_t)seq * kv.table_stride;
+  check(t + from, (to - from + 1) * 4ull, "page table");
+  if (to >= kv.table_stride) hipsim_fail("page table row too short");
+  for (uint32_t i = from; i <= to; ++i) {
+    if (t[i] >= kv.pages) hipsim_fail("page number out of the pool");
+    const uint64_t n = kv.hkv * paged_head_elems(kv.page_log2, d);
+    check((const char*)kv.k + t[i] * n * es, n * es, "page keys");
+    check((const char*)kv.v + t[i] * n * es, n * es, "page values");
+    if (kv.bounds) check((const char*)kv.bounds + (uint64_t)t[i] * kv.hkv * 2 * d * es, kv.hkv * 2 * d * es, "page bounds");
+  }
+}
+
+void check_grid(uint64_t x, uint64_t y, uint64_t z) {
+  if (x == 0 || y == 0 || z == 0 || x > 0x7FFFFFFFu || y > 65535 || z > 65535) hipsim_fail("grid out of range");
+}
+
+}  // namespace
+
+hipError_t launch_paged_table(const PagedTableArgs& a, hipStream_t stream) {
+  return run(stream, "paged_table_kernel", [a] {
+    if (a.count > kTableWrites) hipsim_fail("too many table writes");
+    for (uint32_t i = 0; i < a.count; ++i) {
+      check(a.table + a.at[i], 4, "page table");
+      a.table[a.at[i]] = a.page[i];
+    }
+  });
+}
+
+hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, hipStream_t stream) {
+  return run(stream, "paged_append_kernel", [a, f16, d] {
+    const size_t es = f16 ? 2 : 4;
+    check_grid(a.max_tiles, a.num_heads + 2 * a.kv.hkv, a.chunks);
+    if ((a.q_out == nullptr) != (a.num_heads == 0)) hipsim_fail("query heads without a place for them");
+    for (uint32_t i = 0; i < a.chunks; ++i) {
+      const PagedChunk& c = a.c[i];
+      const uint32_t last = c.start + c.rows - 1;
+      if (last / kTileSlots - c.start / kTileSlots >= a.max_tiles) hipsim_fail("chunk of more tiles than the grid");
+      if ((last >> a.kv.page_log2) - (c.start >> a.kv.page_log2) >= a.max_pages) hipsim_fail("chunk of more pages than the grid");
+      const uint64_t qd = (uint64_t)a.num_heads * d, kd = (uint64_t)a.kv.hkv * d;
+      if (a.q_out) {
+        check(a.q + c.row0 * qd, c.rows * qd * 4, "q");
+        check(a.q_out + c.row0 * qd, c.rows * qd * 4, "rotated q");
+      }
+      check(a.k + c.row0 * kd, c.rows * kd * 4, "k");
+      check(a.v + c.row0 * kd, c.rows * kd * 4, "v");
+      if (a.cos_t) {
+        check(a.cos_t, ((uint64_t)last + 1) * a.pairs * 4, "rope cos");
+        check(a.sin_t, ((uint64_t)last + 1) * a.pairs * 4, "rope sin");
+      }
+      check_pages(a.kv, c.seq, c.start >> a.kv.page_log2, last >> a.kv.page_log2, d, es);
+    }
+  });
+}
+
+hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, uint32_t max_pages, hipStream_t stream) {
+  return run(stream, "paged_select_kernel", [a, f16, d, max_pages] {
+    check_grid((max_pages + a.pages_per_wg - 1) / a.pages_per_wg, (uint64_t)a.max_rows * a.kv.hkv, a.chunks);
+    check(a.keys, (uint64_t)a.chunks * a.max_rows * a.kv.hkv * a.key_stride * 8, "page scores");
+    check(a.tickets, (uint64_t)a.chunks * a.max_rows * a.kv.hkv * 4, "tickets");
+    for (uint64_t i = 0; i < (uint64_t)a.chunks * a.max_rows * a.kv.hkv; ++i)
+      if (a.tickets[i] != 0) hipsim_fail("a ticket is not zero");
+    for (uint32_t i = 0; i < a.chunks; ++i) {
+      const PagedChunk& c = a.c[i];
+      const uint32_t last = (c.start + c.rows - 1) >> a.kv.page_log2;
+      if (c.rows > a.max_rows || last >= a.key_stride || last >= max_pages) hipsim_fail("chunk past the launch's sizes");
+      check(a.q + (uint64_t)c.row0 * a.num_heads * d, (uint64_t)c.rows * a.num_heads * d * 4, "q");
+      check(a.pages + (uint64_t)c.row0 * a.kv.hkv * a.budget, (uint64_t)c.rows * a.kv.hkv * a.budget * 4, "selected pages");
+      check_pages(a.kv, c.seq, 0, last, d, f16 ? 2 : 4);
+    }
+  });
+}
+
+hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, hipStream_t stream) {
+  return run(stream, "paged_attend_kernel", [a, f16, d] {
+    const uint64_t units = (uint64_t)a.max_blocks * a.kv.hkv * a.head_groups;
+    check_grid(a.max_splits, units, a.chunks);
+    if (a.max_splits > 1) {
+      check(a.tickets, units * a.chunks * 4, "tickets");
+      for (uint64_t i = 0; i < units * a.chunks; ++i)
+        if (a.tickets[i] != 0) hipsim_fail("a ticket is not zero");
+    }
+    for (uint32_t i = 0; i < a.chunks; ++i) {
+      const PagedChunk& c = a.c[i];
+      const uint64_t qd = (uint64_t)a.num_heads * d;
+      check(a.q + c.row0 * qd, c.rows * qd * 4, "q");
+      check(a.out + c.row0 * qd, c.rows * qd * 4, "out");
+      if (a.pages) check(a.pages + (uint64_t)c.row0 * a.kv.hkv * a.budget, (uint64_t)c.rows * a.kv.hkv * a.budget * 4, "selected pages");
+      const uint32_t blocks = (c.rows + a.rows_per_block - 1) / a.rows_per_block;
+      if (blocks > a.max_blocks) hipsim_fail("chunk of more blocks than the grid");
+      for (uint32_t b = 0; b < blocks; ++b) {
+        const uint32_t r0 = b * a.rows_per_block, r1 = std::min(r0 + a.rows_per_block, c.rows) - 1;
+        uint32_t t0, t1;
+        paged_range(c.start + r0, c.start + r1, a.window, a.pages ? a.budget : 0, a.kv.page_log2, paged_step(f16), t0, t1);
+        const uint32_t ns = (t1 - t0 + a.tiles_per_split - 1) / a.tiles_per_split;
+        if (ns > c.nsplit || ns > a.max_splits) hipsim_fail("block of more splits than planned");
+      }
+      if (c.nsplit > 1)
+        check(a.part + (uint64_t)c.part0 * kHeadSlots * (d + 4),
+              (uint64_t)blocks * a.kv.hkv * a.head_groups * c.nsplit * kHeadSlots * (d + 4) * 4, "split states");
+      check_pages(a.kv, c.seq, first_visible(c.start, a.window) >> a.kv.page_log2, (c.start + c.rows - 1) >> a.kv.page_log2,
+                  d, f16 ? 2 : 4);
+    }
+  });
+}
+
+hipError_t launch_adapter_load(const AdapterLoadArgs& a, hipStream_t stream) {
+  return run(stream, "adapter_load_kernel", [a] {
+    const uint64_t e = adapter_elem(a.dtype), r16 = adapter_rank16(a.rank);
+    check(a.a, a.rank * (uint64_t)a.cols * e, "A");
+    check(a.b, a.rank * (uint64_t)a.outs * e, "B");
+    check(a.a_to, r16 * a.cols * e, "stored A");
+    check(a.b_to, r16 * a.outs * e, "stored B");
+  });
+}
+
+hipError_t launch_adapter_apply(const AdapterArgs& a, hipStream_t stream) {
+  return run(stream, "adapter_kernels", [a] {
+    const uint64_t e = adapter_elem(a.dtype);
+    check_grid(a.splits, (a.max_rows + 7) / 8, a.runs);
+    if (a.runs > kRunsPerLaunch || (uint64_t)a.splits * a.cols_per_split < a.cols) hipsim_fail("launch does not cover the call");
+    for (uint32_t i = 0; i < a.runs; ++i) {
+      const AdapterRun& r = a.run[i];
+      if (r.rows > a.max_rows || r.rank16 > a.max_rank16) hipsim_fail("run past the launch's sizes");
+      check(a.x + (uint64_t)r.row0 * a.cols, (uint64_t)r.rows * a.cols * 4, "input");
+      if (a.base) check(a.base + (uint64_t)r.row0 * a.outs, (uint64_t)r.rows * a.outs * 4, "base");
+      check(a.out + (uint64_t)r.row0 * a.outs, (uint64_t)r.rows * a.outs * 4, "output");
+      if (r.rank16 == 0) continue;
+      check(a.down + (uint64_t)r.row0 * a.splits * a.max_rank16, (uint64_t)r.rows * a.splits * a.max_rank16 * 4, "products");
+      check((const char*)a.a + r.a_at * e, (uint64_t)r.rank16 * a.cols * e, "stored A");
+      check((const char*)a.b + r.b_at * e, (uint64_t)r.rank16 * a.outs * e, "stored B");
+    }
+  });
 }
 
 }  // namespace jma
