@@ -92,6 +92,9 @@ struct PagedAttendArgs {
 static_assert(sizeof(PagedAttendArgs) <= 4096 && sizeof(PagedAppendArgs) <= 4096,
               "kernel arguments exceed their limit");
 
+// Pages one workgroup of the selection scores.
+constexpr uint32_t kSelectPages = 64;
+
 struct PagedSelectArgs {
   PagedView kv;
   const float* q;      // rotated
@@ -99,7 +102,7 @@ struct PagedSelectArgs {
   uint64_t* keys;      // scratch [row slot][hkv][key_stride]: the pages' scores as ordered integers
   uint32_t* tickets;   // [row slot][hkv], zero between launches
   uint32_t num_heads, group, top, first, last, budget;
-  uint32_t key_stride, pages_per_wg, max_rows;
+  uint32_t key_stride, max_rows;
   uint32_t chunks;
   PagedChunk c[kMaxChunks];
 };

@@ -216,15 +216,203 @@ __device__ __forceinline__ uint64_t ordered(double x) {
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-constexpr uint64_t kAlways = 0xFFFFFFFFFFFFFFFFull;
+// Sum over the 16 lanes of a row, in vector ALU exchanges; every lane gets the same bits.
+template <int kCtrl>
+__device__ __forceinline__ double row_moved(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, kCtrl, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), kCtrl, 0xF, 0xF, false);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double row_sum(double x) {
+  x += row_moved<0x128>(x);  // row_ror by 8, 4, 2, 1
+  x += row_moved<0x124>(x);
+  x += row_moved<0x122>(x);
+  x += row_moved<0x121>(x);
+  return x;
+}
 
-// Workgroup = (group of pages, row x kv head, chunk). Scores: for a page with bounds lo, hi and each
-// query head of the group, sum_d max(q_d lo_d, q_d hi_d), which no key of the page exceeds; the
-// page's score is the largest of the heads'. The sums are formed in 64 bits, where the products are
-// exact, so that which of two nearly equal pages is taken does not depend on the order of a sum.
-// The last workgroup of a (row, kv head) to finish picks the `budget` largest keys, of equal ones
-// the lowest page: it narrows the key of the last page taken by eight bits a pass, then writes the
-// pages in ascending order.
+constexpr uint32_t kPickRounds = 16, kPickPages = 256 * kPickRounds;  // keys a workgroup holds in registers
+
+// The pages of one (row, kv head), ascending: the first `first`, the last `last` and the `top` others of
+// the largest keys, of equal ones the lowest. The key of the last page taken is narrowed by eight
+// bits a pass, from the highest bit in which any two keys differ, until every key that shares the bits
+// found so far is taken (two or three passes: the keys are spread). n > first + last + top.
+__device__ __forceinline__ void pick_pages(const uint64_t* keys, uint32_t n, uint32_t top, uint32_t first, uint32_t last,
+                                           uint32_t* out) {
+  __shared__ uint32_t s_hist[256], s_found[3], s_any[4][2], s_sum[4];
+  __shared__ uint32_t s_count[4 * kPickRounds];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint64_t k[kPickRounds];
+  auto candidate = [&](uint32_t p) JMA_INL { return p >= first && p + last < n; };
+  auto load = [&](uint32_t base) JMA_INL {
+#pragma unroll
+    for (uint32_t i = 0; i < kPickRounds; ++i) {
+      const uint32_t p = base + 256 * i + tid;
+      k[i] = 0;
+      if (base + 256 * i < n && candidate(p)) k[i] = __hip_atomic_load(&keys[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  };
+  auto each = [&](auto&& f) JMA_INL {  // f(round's first page) over the keys, re-read where they are too many
+    for (uint32_t base = 0; base < n; base += kPickPages) {
+      if (n > kPickPages) load(base);
+      f(base);
+    }
+  };
+  load(0);
+
+  // The bits in which the keys differ from the first one's.
+  const uint64_t reference = __hip_atomic_load(&keys[first], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  uint64_t differ = 0;
+  each([&](uint32_t base) JMA_INL {
+#pragma unroll
+    for (uint32_t i = 0; i < kPickRounds; ++i)
+      if (candidate(base + 256 * i + tid)) differ |= k[i] ^ reference;
+  });
+  uint32_t lo = (uint32_t)differ, hi = (uint32_t)(differ >> 32);
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    lo |= __shfl_xor(lo, m);
+    hi |= __shfl_xor(hi, m);
+  }
+  if (lane == 0) s_any[wave][0] = lo, s_any[wave][1] = hi;
+  __syncthreads();
+  differ = (uint64_t)(s_any[0][1] | s_any[1][1] | s_any[2][1] | s_any[3][1]) << 32 | (s_any[0][0] | s_any[1][0] | s_any[2][0] | s_any[3][0]);
+  int shift = differ == 0 ? 0 : max(0, 64 - __clzll((long long)differ) - 8);
+  uint64_t prefix = shift + 8 >= 64 ? 0 : reference >> (shift + 8);  // bits found so far
+  uint32_t need = top;
+  bool all = top == 0 || differ == 0;
+  if (differ == 0) prefix = reference;
+  const bool tie = differ == 0;  // one key throughout: the lowest pages
+  for (; !all; shift = max(0, shift - 8)) {
+    s_hist[tid] = 0;
+    __syncthreads();
+    each([&](uint32_t base) JMA_INL {
+#pragma unroll
+      for (uint32_t i = 0; i < kPickRounds; ++i)
+        if (candidate(base + 256 * i + tid) && (shift + 8 >= 64 || k[i] >> (shift + 8) == prefix))
+          atomicAdd(&s_hist[(k[i] >> shift) & 255], 1u);
+    });
+    __syncthreads();
+    // How many keys are in bin `tid` and above.
+    const uint32_t mine = s_hist[tid];
+    uint32_t above = mine;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const uint32_t x = __shfl_down(above, m);
+      if (lane + m < 64) above += x;
+    }
+    if (lane == 0) s_sum[wave] = above;
+    __syncthreads();
+    for (uint32_t w = wave + 1; w < 4; ++w) above += s_sum[w];
+    if (above >= need && above - mine < need) {
+      s_found[0] = tid;
+      s_found[1] = need - (above - mine);
+      s_found[2] = mine;
+    }
+    __syncthreads();
+    prefix = prefix << 8 | s_found[0];
+    need = s_found[1];
+    all = need == s_found[2] || shift == 0;
+    if (all) break;
+    if (shift < 8) {  // the last pass takes the bits that are left
+      const int left = shift;
+      s_hist[tid] = 0;
+      __syncthreads();
+      each([&](uint32_t base) JMA_INL {
+#pragma unroll
+        for (uint32_t i = 0; i < kPickRounds; ++i)
+          if (candidate(base + 256 * i + tid) && k[i] >> left == prefix) atomicAdd(&s_hist[k[i] & ((1u << left) - 1)], 1u);
+      });
+      __syncthreads();
+      const uint32_t bin = s_hist[tid];
+      uint32_t up = bin;
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const uint32_t x = __shfl_down(up, m);
+        if (lane + m < 64) up += x;
+      }
+      if (lane == 0) s_sum[wave] = up;
+      __syncthreads();
+      for (uint32_t w = wave + 1; w < 4; ++w) up += s_sum[w];
+      if (up >= need && up - bin < need) {
+        s_found[0] = tid;
+        s_found[1] = need - (up - bin);
+        s_found[2] = bin;
+      }
+      __syncthreads();
+      prefix = prefix << left | s_found[0];
+      need = s_found[1];
+      shift = 0;
+      break;
+    }
+  }
+  // Taken: keys above the last one's bits, and of those that share them the lowest `need` pages (all of
+  // them unless keys are equal).
+  uint32_t taken = 0, equal = 0;  // before this round of kPickPages pages
+  each([&](uint32_t base) JMA_INL {
+    uint32_t flags = 0, ties = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kPickRounds; ++i) {
+      const uint32_t p = base + 256 * i + tid;
+      const uint64_t x = tie ? k[i] : k[i] >> shift;
+      const bool c = candidate(p), eq = c && top != 0 && x == prefix;
+      if (p < n && (!c || (top != 0 && x > prefix))) flags |= 1u << i;
+      if (eq) ties |= 1u << i;
+    }
+    // Ranks of the equal keys, in page order.
+    auto ranks = [&](uint32_t set, uint32_t before, uint32_t* total) JMA_INL {
+      __syncthreads();
+#pragma unroll
+      for (uint32_t i = 0; i < kPickRounds; ++i) {
+        const uint64_t b = __ballot((set >> i) & 1);
+        if (lane == 0) s_count[4 * i + wave] = __popcll(b);
+      }
+      __syncthreads();
+      if (wave == 0) {
+        const uint32_t mine = s_count[lane];
+        uint32_t sum = mine;
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) {
+          const uint32_t x = __shfl_up(sum, m);
+          if (lane >= (uint32_t)m) sum += x;
+        }
+        s_count[lane] = sum - mine;
+        if (lane == 63) s_sum[0] = sum;
+      }
+      __syncthreads();
+      *total = before + s_sum[0];
+      return before;
+    };
+    auto rank = [&](uint32_t set, uint32_t i, uint32_t before) JMA_INL {
+      const uint64_t b = __ballot((set >> i) & 1);
+      return before + s_count[4 * i + wave] + (uint32_t)__popcll(b & ((1ull << lane) - 1));
+    };
+    uint32_t next;
+    const uint32_t before_eq = ranks(ties, equal, &next);
+#pragma unroll
+    for (uint32_t i = 0; i < kPickRounds; ++i) {
+      const uint32_t r = rank(ties, i, before_eq);
+      if (((ties >> i) & 1) && r < need) flags |= 1u << i;
+    }
+    equal = next;
+    const uint32_t before = ranks(flags, taken, &next);
+#pragma unroll
+    for (uint32_t i = 0; i < kPickRounds; ++i) {
+      const uint32_t r = rank(flags, i, before);
+      if ((flags >> i) & 1) out[r] = base + 256 * i + tid;
+    }
+    taken = next;
+  });
+}
+
+// Workgroup = (64 pages, row x kv head, chunk). Scores: for a page with bounds lo, hi and each query
+// head of the group, sum_d max(q_d lo_d, q_d hi_d), which no key of the page exceeds; the page's score
+// is the largest of the heads'. The sums are formed in 64 bits, where the products are exact, so that
+// which of two nearly equal pages is taken does not depend on the order of a sum. 16 lanes take a page,
+// four pages each, whose table entries and bounds are all in flight before the first is used: the
+// kernel's time is those two memory round trips and the pick's, not its arithmetic (64 pages, 4 heads of
+// 128: 1 us). The last workgroup of a (row, kv head) to finish picks the pages.
 template <typename KV, int D>
 __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs a) {
   const PagedChunk c = a.c[blockIdx.z];
@@ -232,11 +420,10 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   if (r >= c.rows) return;
   const uint32_t pos = c.start + r, row = c.row0 + r;
   const uint32_t n = (pos >> a.kv.page_log2) + 1;
-  const uint32_t first_page = blockIdx.x * a.pages_per_wg;
+  const uint32_t first_page = blockIdx.x * kSelectPages;
   if (first_page >= n) return;
-  const uint32_t wgs = (n + a.pages_per_wg - 1) / a.pages_per_wg;
+  const uint32_t wgs = (n + kSelectPages - 1) / kSelectPages;
   uint32_t* out = a.pages + ((uint64_t)row * hkv + kvh) * a.budget;
-  __shared__ uint32_t s_last;
   if (n <= a.budget) {  // every page
     if (blockIdx.x == 0)
       for (uint32_t i = threadIdx.x; i < a.budget; i += 256) out[i] = i < n ? i : kNoPage;
@@ -245,112 +432,57 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   const uint64_t slot = ((uint64_t)blockIdx.z * a.max_rows + r) * hkv + kvh;
   uint64_t* keys = a.keys + slot * a.key_stride;
 
-  // 16 lanes take a page, D / 16 elements each.
-  constexpr int kE = D / 16;
-  const uint32_t lane16 = threadIdx.x % 16;
-  const float* q = a.q + ((uint64_t)row * a.num_heads + kvh * a.group) * D + lane16 * kE;
-  const uint32_t last_page = min(first_page + a.pages_per_wg, n);
-  for (uint32_t p = first_page + threadIdx.x / 16; p < last_page; p += 16) {
-    uint64_t key = kAlways;
-    if (p >= a.first && p + a.last < n) {
-      const uint32_t page = a.kv.table[(uint64_t)c.seq * a.kv.table_stride + p];
-      const KV* b = (const KV*)a.kv.bounds + ((uint64_t)page * hkv + kvh) * 2 * D + lane16 * kE;
-      double lo[kE], hi[kE];
+  constexpr int kE = D / 16, kP = kSelectPages / 16;
+  typedef KV kve_t __attribute__((ext_vector_type(kE)));
+  const uint32_t lane16 = threadIdx.x % 16, own = threadIdx.x / 16;
+  const uint32_t* table = a.kv.table + (uint64_t)c.seq * a.kv.table_stride;
+  uint32_t page[kP];
 #pragma unroll
-      for (int e = 0; e < kE; ++e) lo[e] = (double)(float)b[e], hi[e] = (double)(float)b[D + e];
-      double best = -INFINITY;
-      bool odd = false;
-      for (uint32_t h = 0; h < a.group; ++h) {
-        double s = 0.0;
+  for (int i = 0; i < kP; ++i) page[i] = table[min(first_page + 16 * i + own, n - 1)];
+  kve_t lo[kP], hi[kP];
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          const float x = q[(uint64_t)h * D + e];
-          s = fma((double)x, x >= 0.0f ? hi[e] : lo[e], s);
-        }
-#pragma unroll
-        for (int m = 1; m < 16; m *= 2) s += __shfl_xor(s, m, 16);
-        odd = odd || s != s;
-        best = s > best ? s : best;
-      }
-      key = odd ? kAlways : ordered(best);
-    }
-    if (lane16 == 0) __hip_atomic_store(&keys[p], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = 0; i < kP; ++i) {
+    const KV* b = (const KV*)a.kv.bounds + ((uint64_t)page[i] * hkv + kvh) * 2 * D + lane16 * kE;
+    lo[i] = *(const kve_t*)b;
+    hi[i] = *(const kve_t*)(b + D);
   }
+  const float* q = a.q + ((uint64_t)row * a.num_heads + kvh * a.group) * D + lane16 * kE;
+  double best[kP];
+  bool odd[kP];
+#pragma unroll
+  for (int i = 0; i < kP; ++i) best[i] = -INFINITY, odd[i] = false;
+  for (uint32_t h = 0; h < a.group; ++h) {
+    float x[kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) x[e] = q[(uint64_t)h * D + e];
+#pragma unroll
+    for (int i = 0; i < kP; ++i) {
+      double s = 0.0;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) s = fma((double)x[e], (double)(float)(x[e] >= 0.0f ? hi[i][e] : lo[i][e]), s);
+      s = row_sum(s);
+      odd[i] = odd[i] || s != s;
+      best[i] = s > best[i] ? s : best[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kP; ++i) {
+    const uint32_t p = first_page + 16 * i + own;
+    if (lane16 == 0 && p < n)
+      __hip_atomic_store(&keys[p], odd[i] ? 0xFFFFFFFFFFFFFFFFull : ordered(best[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  // The keys are acknowledged (visible device-wide) before the ticket is taken.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
   if (wgs > 1) {
-    // The keys are acknowledged (visible device-wide) before the ticket is taken.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    __shared__ uint32_t s_last;
     if (threadIdx.x == 0)
       s_last = __hip_atomic_fetch_add(&a.tickets[slot], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (s_last + 1 != wgs) return;
     if (threadIdx.x == 0) __hip_atomic_store(&a.tickets[slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  } else {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
   }
-
-  __shared__ uint32_t s_hist[256], s_at, s_need, s_wave[4];
-  auto key_of = [&](uint32_t p) JMA_INL {
-    return __hip_atomic_load(&keys[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  };
-  uint64_t prefix = 0;       // the leading bits of the last key taken
-  uint32_t need = a.budget;  // keys still to take among those with that prefix
-  int shift = 56;
-  for (; shift >= 0; shift -= 8) {
-    s_hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (uint32_t p = threadIdx.x; p < n; p += 256) {
-      const uint64_t k = key_of(p);
-      if (shift == 56 || k >> (shift + 8) == prefix) atomicAdd(&s_hist[(k >> shift) & 255], 1u);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint32_t left = need, d = 255;
-      while (d > 0 && s_hist[d] < left) left -= s_hist[d--];
-      s_at = d;
-      s_need = left;
-    }
-    __syncthreads();
-    prefix = (prefix << 8) | s_at;
-    need = s_need;
-    const bool all = s_hist[s_at] == need;  // every key with this prefix is taken
-    __syncthreads();
-    if (all) break;
-  }
-  // Taken: keys above the prefix's range, and the lowest `need` pages inside it.
-  const int low = shift < 0 ? 0 : shift;
-  uint32_t taken = 0, inside = 0;  // so far, over all pages before this round's
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (uint32_t p0 = 0; p0 < n; p0 += 256) {
-    const uint32_t p = p0 + threadIdx.x;
-    const uint64_t k = p < n ? key_of(p) >> low : 0;
-    const bool eq = p < n && k == prefix;
-    const uint64_t eqs = __ballot(eq);
-    if (lane == 0) s_wave[wave] = __popcll(eqs);
-    __syncthreads();
-    uint32_t before = inside, total_eq = 0;
-    for (uint32_t w = 0; w < 4; ++w) {
-      if (w < wave) before += s_wave[w];
-      total_eq += s_wave[w];
-    }
-    before += __popcll(eqs & ((1ull << lane) - 1));
-    const bool take = p < n && (k > prefix || (eq && before < need));
-    const uint64_t takes = __ballot(take);
-    __syncthreads();
-    if (lane == 0) s_wave[wave] = __popcll(takes);
-    __syncthreads();
-    uint32_t at = taken, total = 0;
-    for (uint32_t w = 0; w < 4; ++w) {
-      if (w < wave) at += s_wave[w];
-      total += s_wave[w];
-    }
-    at += __popcll(takes & ((1ull << lane) - 1));
-    if (take) out[at] = p;
-    taken += total;
-    inside += total_eq;
-    __syncthreads();
-  }
+  pick_pages(keys, n, a.top, a.first, a.last, out);
 }
 
 // ================================================================ attention
@@ -779,7 +911,7 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, u
   return by_shape(f16, d, [&](auto kv, auto dim) {
     using KV = decltype(kv);
     constexpr int D = decltype(dim)::value;
-    const uint32_t wgs = (max_pages + a.pages_per_wg - 1) / a.pages_per_wg;
+    const uint32_t wgs = (max_pages + kSelectPages - 1) / kSelectPages;
     paged_select_kernel<KV, D><<<dim3(wgs, a.max_rows * a.kv.hkv, a.chunks), 256, 0, stream>>>(a);
     return hipGetLastError();
   });

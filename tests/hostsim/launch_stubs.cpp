@@ -334,7 +334,7 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, h
 
 hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, uint32_t max_pages, hipStream_t stream) {
   return run(stream, "paged_select_kernel", [a, f16, d, max_pages] {
-    check_grid((max_pages + a.pages_per_wg - 1) / a.pages_per_wg, (uint64_t)a.max_rows * a.kv.hkv, a.chunks);
+    check_grid((max_pages + kSelectPages - 1) / kSelectPages, (uint64_t)a.max_rows * a.kv.hkv, a.chunks);
     check(a.keys, (uint64_t)a.chunks * a.max_rows * a.kv.hkv * a.key_stride * 8, "page scores");
     check(a.tickets, (uint64_t)a.chunks * a.max_rows * a.kv.hkv * 4, "tickets");
     for (uint64_t i = 0; i < (uint64_t)a.chunks * a.max_rows * a.kv.hkv; ++i)
