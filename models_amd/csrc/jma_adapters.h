@@ -10,21 +10,25 @@
 
 namespace jma {
 
-constexpr uint32_t kMaxRuns = 128;      // runs of rows one launch takes in its kernel arguments
 constexpr uint32_t kMaxRank = 256;
 constexpr uint32_t kNoAdapter = 0xFFFFFFFFu;
 constexpr uint32_t kAdapterF32 = 0, kAdapterF16 = 1, kAdapterBF16 = 2;
 
 JMA_HD uint32_t adapter_elem(uint32_t dtype) { return dtype == kAdapterF32 ? 4u : 2u; }
-// Ranks are stored rounded up to 16 with zeros: A [rank16][cols], B [outs][rank16].
+// Ranks are stored rounded up to 16 with zeros: A [rank16][cols], and B, whose products read eight ranks
+// of neighbouring outputs, [rank16 / 8][outs][8].
 JMA_HD uint32_t adapter_rank16(uint32_t rank) { return (rank + 15u) & ~15u; }
+JMA_HD uint64_t adapter_b_index(uint64_t out, uint32_t r, uint32_t outs) {
+  return ((uint64_t)(r / 8) * outs + out) * 8 + r % 8;
+}
 
-// `rows` rows from row0 on, adapter at element offset `at` of the weights (rank16 0: none).
+// `rows` rows from row0 on, adapter at element offsets a_at, b_at of the weights (rank16 0: none).
 struct AdapterRun {
   uint32_t rows, row0, rank16;
   float scale;
   uint64_t a_at, b_at;
 };
+constexpr uint32_t kMaxRuns = 96;  // runs of rows one launch takes in its kernel arguments
 
 struct AdapterArgs {
   const void* a;       // the adapters' A and B weights
@@ -32,22 +36,36 @@ struct AdapterArgs {
   const float* x;      // [rows][cols]
   const float* base;   // [rows][outs], may be out; null: zero
   float* out;
-  float* down;         // scratch [rows][splits][max_rank16]
-  uint32_t dtype, cols, outs, max_rank16, splits, cols_per_split, max_rows, runs;
-  AdapterRun run[kMaxRuns - 32];
+  float* down;         // scratch [rows][splits][max_rank16] of the two-launch form
+  uint32_t dtype, cols, outs, max_rank16;
+  uint32_t splits, cols_per_split;  // pieces of the columns in the two-launch form
+  uint32_t row_block;               // rows of one workgroup in the one-launch form
+  uint32_t max_rows, runs;
+  AdapterRun run[kMaxRuns];
 };
-constexpr uint32_t kRunsPerLaunch = kMaxRuns - 32;
 static_assert(sizeof(AdapterArgs) <= 4096, "kernel arguments exceed their limit");
 
 struct AdapterLoadArgs {
   const void* a;  // [rank][cols]
   const void* b;  // [outs][rank]
-  void* a_to;     // [rank16][cols]
-  void* b_to;     // [outs][rank16]
+  void* a_to;
+  void* b_to;
   uint32_t dtype, rank, cols, outs;
 };
 
-// Columns one workgroup of the first product takes: at least 256, at most 8 pieces a row.
-inline uint32_t adapter_splits(uint32_t cols) { return std::max(1u, std::min(8u, cols / 256)); }
+// Outputs of a workgroup of the one-launch form, and the LDS floats its input rows may take.
+constexpr uint32_t kFewOuts = 512, kFewFloats = 14336;
+// Rows one workgroup takes in the one-launch form (0: the columns do not fit).
+JMA_HD uint32_t adapter_few_rows(uint32_t cols) {
+  const uint32_t fit = kFewFloats / cols;
+  return fit < 4u ? fit : 4u;
+}
+// Rows and outputs of a workgroup's tile in the two-launch form.
+constexpr uint32_t kDownRows = 32, kUpRows = 64, kUpOuts = 128;
+// Pieces of the columns, so that few row blocks still fill the compute units: at least 256 columns each.
+inline uint32_t adapter_splits(uint32_t cols, uint64_t row_blocks, uint32_t cus) {
+  const uint64_t want = (2ull * cus + row_blocks - 1) / std::max<uint64_t>(row_blocks, 1);
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({want, 16ull, std::max(1u, cols / 256)}));
+}
 
 }  // namespace jma

@@ -1,5 +1,12 @@
 // gfx950 kernels of low-rank adapters beside a shared projection: out = base + scale B (A x), each run
 // of rows with an adapter of its own.
+//
+//   adapter_few_kernel    runs of few rows, one launch: every workgroup forms all of A x for its rows
+//   adapter_down_kernel   longer runs: A x on the f32 matrix cores, split over the columns
+//   adapter_up_kernel     base + scale B (A x) on the f32 matrix cores
+//
+// Inputs, sums and outputs are 32-bit, weights are widened exactly, so the result is that of 32-bit
+// arithmetic for every weight type; sums are formed in a fixed order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -12,106 +19,278 @@ namespace {
 
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 
 #define JMA_INL __attribute__((always_inline))
 
-// Rows of a run that share a workgroup's weight loads.
-constexpr uint32_t kRowBlock = 8;
-
-// Eight weights, widened exactly.
-template <uint32_t kType>
-__device__ __forceinline__ void load8(const void* p, uint64_t at, float (&w)[8]) {
-  if constexpr (kType == kAdapterF32) {
-    const float4_t x = *(const float4_t*)((const float*)p + at), y = *(const float4_t*)((const float*)p + at + 4);
+// N (4 or 8) weights as they are stored, and widened.
+template <uint32_t kType, int N>
+struct Raw {
+  static constexpr int kWords = kType == kAdapterF32 ? N : N / 2;
+  typedef uint32_t words_t __attribute__((ext_vector_type(kWords)));
+  words_t w;
+  __device__ __forceinline__ void load(const void* p, uint64_t at) {
+    const char* q = (const char*)p + at * adapter_elem(kType);
+    if constexpr (kWords == 8) {
+      const uint4_t x = *(const uint4_t*)q, y = *(const uint4_t*)(q + 16);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = x[e], w[4 + e] = y[e];
-  } else if constexpr (kType == kAdapterF16) {
-    typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-    const half8_t x = *(const half8_t*)((const _Float16*)p + at);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = (float)x[e];
-  } else {
-    const uint4_t x = *(const uint4_t*)((const uint16_t*)p + at);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      w[2 * e] = __uint_as_float(x[e] << 16);
-      w[2 * e + 1] = __uint_as_float(x[e] & 0xFFFF0000u);
+      for (int i = 0; i < 4; ++i) w[i] = x[i], w[4 + i] = y[i];
+    } else {
+      w = *(const words_t*)q;
     }
   }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (kType == kAdapterF32) return __uint_as_float(w[i]);
+    else if constexpr (kType == kAdapterBF16) return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2]));
+  }
+};
+
+template <int kCtrl>
+__device__ __forceinline__ float moved(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), kCtrl, 0xF, 0xF, false));
+}
+// Sum over the wave's 64 lanes; every lane gets the same bits.
+__device__ __forceinline__ float wave_sum(float x) {
+  x += moved<0x128>(x);  // row_ror by 8, 4, 2, 1
+  x += moved<0x124>(x);
+  x += moved<0x122>(x);
+  x += moved<0x121>(x);
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Workgroup = (piece of the columns, block of a run's rows, run): A x over that piece, for every rank.
-// A wave takes a rank at a time, its lanes eight columns each; sums are 32-bit, in a fixed tree.
-template <uint32_t kType>
-__global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterArgs a) {
+// Workgroup = (512 outputs, block of kRows rows, run). Every workgroup forms all of A x for its rows: A
+// comes from the L2 for all but the first, and a second launch, which would have to wait for the first,
+// costs more than reading it again (2048 columns and outputs: one row of rank 16 9.1 us as two launches,
+// 5.5 as one; 64 rows of 40 adapters of ranks 8 to 64 24.7 and 11.0). A wave takes two ranks at a time, its lanes
+// eight columns each of every 512; then a thread takes an output.
+template <uint32_t kType, int kRows>
+__global__ __launch_bounds__(512) void adapter_few_kernel(const AdapterArgs a) {
   const AdapterRun run = a.run[blockIdx.z];
-  const uint32_t r0 = blockIdx.y * kRowBlock;
-  if (run.rank16 == 0 || r0 >= run.rows) return;
-  const uint32_t rows = min(kRowBlock, run.rows - r0);
-  const uint32_t c0 = blockIdx.x * a.cols_per_split, c1 = min(c0 + a.cols_per_split, a.cols);
+  const uint32_t r0 = blockIdx.y * kRows;
+  if (r0 >= run.rows) return;
+  const uint32_t rows = min((uint32_t)kRows, run.rows - r0);
+  extern __shared__ __attribute__((aligned(16))) float s_x[];  // [kRows][cols]
+  __shared__ __attribute__((aligned(16))) float s_down[kRows][kMaxRank];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float* x = a.x + (uint64_t)(run.row0 + r0) * a.cols;
-  for (uint32_t r = wave; r < run.rank16; r += 4) {
-    float sum[kRowBlock] = {};
-    for (uint32_t c = c0 + 8 * lane; c < c1; c += 512) {
-      float w[8];
-      load8<kType>(a.a, run.a_at + (uint64_t)r * a.cols + c, w);
+  const uint32_t o = blockIdx.x * kFewOuts + threadIdx.x;
+  const uint64_t at = (uint64_t)(run.row0 + r0) * a.outs + o;
+  if (run.rank16 != 0) {
+    const float* x = a.x + (uint64_t)(run.row0 + r0) * a.cols;
+    for (uint32_t i = threadIdx.x; i < rows * (a.cols / 4); i += 512) *(float4_t*)&s_x[4 * i] = *(const float4_t*)(x + 4 * i);
+    __syncthreads();
+    for (uint32_t r = 2 * wave; r < run.rank16; r += 16) {
+      float sum[2][kRows] = {};
+      auto take = [&](const Raw<kType, 8>& w0, const Raw<kType, 8>& w1, uint32_t c) JMA_INL {
 #pragma unroll
-      for (uint32_t i = 0; i < kRowBlock; ++i) {
-        if (i >= rows) continue;
-        const float4_t u = *(const float4_t*)(x + (uint64_t)i * a.cols + c), v = *(const float4_t*)(x + (uint64_t)i * a.cols + c + 4);
+        for (int i = 0; i < kRows; ++i) {
+          if (i > 0 && (uint32_t)i >= rows) continue;
+          const float4_t u = *(const float4_t*)&s_x[i * a.cols + c], v = *(const float4_t*)&s_x[i * a.cols + c + 4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sum[i] = fmaf(w[e], u[e], sum[i]);
-          sum[i] = fmaf(w[4 + e], v[e], sum[i]);
+          for (int e = 0; e < 4; ++e) {
+            sum[0][i] = fmaf(w0[e], u[e], sum[0][i]);
+            sum[1][i] = fmaf(w1[e], u[e], sum[1][i]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sum[0][i] = fmaf(w0[4 + e], v[e], sum[0][i]);
+            sum[1][i] = fmaf(w1[4 + e], v[e], sum[1][i]);
+          }
+        }
+      };
+      const uint64_t row = run.a_at + (uint64_t)r * a.cols;
+      uint32_t c = 8 * lane;
+      for (; c + 3 * 512 < a.cols; c += 4 * 512) {  // eight loads in flight
+        Raw<kType, 8> w0[4], w1[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w0[i].load(a.a, row + c + 512 * i);
+          w1[i].load(a.a, row + a.cols + c + 512 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) take(w0[i], w1[i], c + 512 * i);
+      }
+      for (; c < a.cols; c += 512) {
+        Raw<kType, 8> w0, w1;
+        w0.load(a.a, row + c);
+        w1.load(a.a, row + a.cols + c);
+        take(w0, w1, c);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const float d0 = wave_sum(sum[0][i]), d1 = wave_sum(sum[1][i]);
+        if (lane == 0) {
+          s_down[i][r] = d0 * run.scale;
+          s_down[i][r + 1] = d1 * run.scale;
         }
       }
     }
+    __syncthreads();
+  }
+  if (o >= a.outs) return;
+  float sum[kRows] = {};
+  for (uint32_t r = 0; r < run.rank16; r += 16) {
+    Raw<kType, 8> w0, w1;
+    w0.load(a.b, run.b_at + adapter_b_index(o, r, a.outs));
+    w1.load(a.b, run.b_at + adapter_b_index(o, r + 8, a.outs));
 #pragma unroll
-    for (uint32_t i = 0; i < kRowBlock; ++i) {
-      if (i >= rows) continue;
+    for (int i = 0; i < kRows; ++i)
 #pragma unroll
-      for (int m = 32; m >= 1; m /= 2) sum[i] += __shfl_xor(sum[i], m);
-      if (lane == 0) a.down[((uint64_t)(run.row0 + r0 + i) * a.splits + blockIdx.x) * a.max_rank16 + r] = sum[i];
+      for (int e = 0; e < 8; ++e) {
+        sum[i] = fmaf(w0[e], s_down[i][r + e], sum[i]);
+        sum[i] = fmaf(w1[e], s_down[i][r + 8 + e], sum[i]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i)
+    if ((uint32_t)i < rows) a.out[at + (uint64_t)i * a.outs] = (a.base ? a.base[at + (uint64_t)i * a.outs] : 0.0f) + sum[i];
+}
+
+// Workgroup = (piece of the columns, 32 rows of a run, run): A x over that piece. Its four waves take a
+// quarter of the piece each and meet in LDS. One 16x16x4 product takes 16 ranks x 16 rows over four
+// columns; lane (g, c) holds eight neighbouring columns 8g .. 8g+7 of its row of either operand per step of
+// 32, so both are read in wide loads. Bound by reading x: ranks are taken 64 at a time, which is all of
+// them for most adapters.
+template <uint32_t kType>
+__global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterArgs a) {
+  const AdapterRun run = a.run[blockIdx.z];
+  const uint32_t r0 = blockIdx.y * kDownRows;
+  if (run.rank16 == 0 || r0 >= run.rows) return;
+  const uint32_t rows = min(kDownRows, run.rows - r0);
+  const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t c0 = blockIdx.x * a.cols_per_split, c1 = min(c0 + a.cols_per_split, a.cols);
+  const uint32_t quarter = ((c1 - c0 + 3) / 4 + 31) / 32 * 32;
+  const uint32_t w0 = min(c0 + wave * quarter, c1), w1 = min(w0 + quarter, c1);
+  __shared__ __attribute__((aligned(16))) float s_part[4][2][4][64][4];  // [wave][row tile][rank tile][lane]
+  // Rows behind the run's last repeat it; their columns of the product are not stored.
+  const float* x[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) x[t] = a.x + (uint64_t)(run.row0 + r0 + min(16u * t + c16, rows - 1)) * a.cols + 8 * g;
+  for (uint32_t rank0 = 0; rank0 < run.rank16; rank0 += 64) {
+    const uint32_t tiles = min(4u, (run.rank16 - rank0) / 16);
+    float4_t acc[2][4] = {};
+    auto step = [&](uint32_t c, auto whole) JMA_INL {
+      float4_t v[2][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          v[t][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+          if (decltype(whole)::value || c + 8 * g < w1) v[t][i] = *(const float4_t*)(x[t] + c + 4 * i);
+        }
+      Raw<kType, 8> w[4];
+#pragma unroll
+      for (uint32_t n = 0; n < 4; ++n) {
+        w[n].w = {};
+        if (n < tiles && (decltype(whole)::value || c + 8 * g < w1))
+          w[n].load(a.a, run.a_at + (uint64_t)(rank0 + 16 * n + c16) * a.cols + c + 8 * g);
+      }
+#pragma unroll
+      for (uint32_t n = 0; n < 4; ++n) {
+        if (n >= tiles) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[n][e], v[t][e / 4][e % 4], acc[t][n], 0, 0, 0);
+      }
+    };
+    uint32_t c = w0;
+    for (; c + 32 <= w1; c += 32) step(c, std::true_type{});
+    if (c < w1) step(c, std::false_type{});
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (uint32_t n = 0; n < 4; ++n) *(float4_t*)s_part[wave][t][n][lane] = acc[t][n];
+    __syncthreads();
+    // Lane (g, c) of a tile holds ranks 4g .. 4g+3 of row c.
+    for (uint32_t i = threadIdx.x; i < 2 * tiles * 64; i += 256) {
+      const uint32_t l = i % 64, n = i / 64 % tiles, t = i / 64 / tiles, row = 16 * t + (l & 15);
+      float4_t sum = *(const float4_t*)s_part[0][t][n][l];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) sum += *(const float4_t*)s_part[w][t][n][l];
+      if (row < rows)
+        *(float4_t*)&a.down[((uint64_t)(run.row0 + r0 + row) * a.splits + blockIdx.x) * a.max_rank16 + rank0 + 16 * n + 4 * (l >> 4)] = sum;
     }
   }
 }
 
-// Workgroup = (256 outputs, block of a run's rows, run): base + scale B (A x), the pieces of A x summed
-// in order.
+// Workgroup = (128 outputs, 64 rows of a run, run): base + scale B (A x), the pieces of A x summed in order
+// into LDS first. A wave takes 32 outputs; a 16x16x4 product leaves lane (g, c) four neighbouring outputs
+// of row c, one 16-byte access each of base and out. Bound by reading base and writing out.
 template <uint32_t kType>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterArgs a) {
   const AdapterRun run = a.run[blockIdx.z];
-  const uint32_t r0 = blockIdx.y * kRowBlock;
+  const uint32_t r0 = blockIdx.y * kUpRows;
   if (r0 >= run.rows) return;
-  const uint32_t rows = min(kRowBlock, run.rows - r0);
-  __shared__ __attribute__((aligned(16))) float s_down[kRowBlock][kMaxRank];
-  for (uint32_t i = threadIdx.x; i < rows * run.rank16; i += 256) {
-    const uint32_t row = i / run.rank16, r = i % run.rank16;
-    const float* p = a.down + (uint64_t)(run.row0 + r0 + row) * a.splits * a.max_rank16 + r;
-    float sum = 0.0f;
-    for (uint32_t s = 0; s < a.splits; ++s) sum += p[(uint64_t)s * a.max_rank16];
-    s_down[row][r] = sum * run.scale;
+  const uint32_t rows = min(kUpRows, run.rows - r0);
+  const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15, wave = threadIdx.x >> 6;
+  const uint32_t o0 = blockIdx.x * kUpOuts + 32 * wave;
+  __shared__ __attribute__((aligned(16))) float s_down[kUpRows][64 + 4];
+  float4_t acc[4][2] = {}, base[4][2];  // [row tile][output tile]
+  const bool wide = a.outs % 4 == 0;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      base[t][n] = float4_t{0.f, 0.f, 0.f, 0.f};
+      const uint32_t row = 16 * t + c16, o = o0 + 16 * n + 4 * g;
+      if (a.base == nullptr || row >= rows || o >= a.outs) continue;
+      const float* p = a.base + (uint64_t)(run.row0 + r0 + row) * a.outs + o;
+      if (wide) base[t][n] = *(const float4_t*)p;
+      else
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+          if (o + e < a.outs) base[t][n][e] = p[e];
+    }
+  for (uint32_t rank0 = 0; rank0 < run.rank16; rank0 += 64) {
+    const uint32_t ranks = min(64u, run.rank16 - rank0);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kUpRows * (ranks / 4); i += 256) {
+      const uint32_t row = i / (ranks / 4), r = 4 * (i % (ranks / 4));
+      float4_t sum = {0.f, 0.f, 0.f, 0.f};
+      if (row < rows) {
+        const float* p = a.down + (uint64_t)(run.row0 + r0 + row) * a.splits * a.max_rank16 + rank0 + r;
+        for (uint32_t s = 0; s < a.splits; ++s) sum += *(const float4_t*)(p + (uint64_t)s * a.max_rank16);
+      }
+      *(float4_t*)&s_down[row][r] = sum * run.scale;
+    }
+    __syncthreads();
+    for (uint32_t r = 0; r < ranks; r += 16) {
+      Raw<kType, 4> w[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        w[n].load(a.b, run.b_at + adapter_b_index(min(o0 + 16 * n + c16, a.outs - 1), rank0 + r + 4 * g, a.outs));
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float4_t d = *(const float4_t*)&s_down[16 * t + c16][r + 4 * g];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[n][e], d[e], acc[t][n], 0, 0, 0);
+      }
+    }
   }
-  __syncthreads();
-  const uint32_t o = blockIdx.x * 256 + threadIdx.x;
-  if (o >= a.outs) return;
-  float sum[kRowBlock];
-  const uint64_t at = (uint64_t)(run.row0 + r0) * a.outs + o;
 #pragma unroll
-  for (uint32_t i = 0; i < kRowBlock; ++i) sum[i] = 0.0f;
-  for (uint32_t r = 0; r < run.rank16; r += 8) {
-    float w[8];
-    load8<kType>(a.b, run.b_at + (uint64_t)o * run.rank16 + r, w);
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (uint32_t i = 0; i < kRowBlock; ++i)
-      if (i < rows)
+    for (int n = 0; n < 2; ++n) {
+      const uint32_t row = 16 * t + c16, o = o0 + 16 * n + 4 * g;
+      if (row >= rows || o >= a.outs) continue;
+      float* p = a.out + (uint64_t)(run.row0 + r0 + row) * a.outs + o;
+      const float4_t y = base[t][n] + acc[t][n];
+      if (wide) *(float4_t*)p = y;
+      else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[i] = fmaf(w[e], s_down[i][r + e], sum[i]);
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < kRowBlock; ++i)
-    if (i < rows) a.out[at + (uint64_t)i * a.outs] = (a.base ? a.base[at + (uint64_t)i * a.outs] : 0.0f) + sum[i];
+        for (uint32_t e = 0; e < 4; ++e)
+          if (o + e < a.outs) p[e] = y[e];
+    }
 }
 
 // An adapter's weights into their stored form, the ranks behind its own zero.
@@ -123,10 +302,18 @@ __global__ __launch_bounds__(256) void adapter_load_kernel(const AdapterLoadArgs
     if (i < na) {
       ((T*)a.a_to)[i] = i / a.cols < a.rank ? ((const T*)a.a)[i] : (T)0;
     } else {
-      const uint64_t j = i - na, o = j / r16, r = j % r16;
-      ((T*)a.b_to)[j] = r < a.rank ? ((const T*)a.b)[o * a.rank + r] : (T)0;
+      const uint64_t j = i - na, o = j / r16;
+      const uint32_t r = (uint32_t)(j % r16);
+      ((T*)a.b_to)[adapter_b_index(o, r, a.outs)] = r < a.rank ? ((const T*)a.b)[o * a.rank + r] : (T)0;
     }
   }
+}
+
+template <typename F>
+hipError_t by_type(uint32_t dtype, F&& f) {
+  if (dtype == kAdapterF32) return f(std::integral_constant<uint32_t, kAdapterF32>{});
+  if (dtype == kAdapterF16) return f(std::integral_constant<uint32_t, kAdapterF16>{});
+  return f(std::integral_constant<uint32_t, kAdapterBF16>{});
 }
 
 }  // namespace
@@ -137,18 +324,27 @@ hipError_t launch_adapter_load(const AdapterLoadArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_adapter_apply(const AdapterArgs& a, hipStream_t stream) {
-  const uint32_t blocks = (a.max_rows + kRowBlock - 1) / kRowBlock;
-  const dim3 down(a.splits, blocks, a.runs), up((a.outs + 255) / 256, blocks, a.runs);
-  auto go = [&](auto type) {
+hipError_t launch_adapter_few(const AdapterArgs& a, hipStream_t stream) {
+  const dim3 grid((a.outs + kFewOuts - 1) / kFewOuts, (a.max_rows + a.row_block - 1) / a.row_block, a.runs);
+  const uint32_t lds = a.row_block * a.cols * 4;
+  return by_type(a.dtype, [&](auto type) {
     constexpr uint32_t kType = decltype(type)::value;
-    adapter_down_kernel<kType><<<down, 256, 0, stream>>>(a);
+    if (a.row_block == 1) adapter_few_kernel<kType, 1><<<grid, 512, lds, stream>>>(a);
+    else if (a.row_block == 2) adapter_few_kernel<kType, 2><<<grid, 512, lds, stream>>>(a);
+    else adapter_few_kernel<kType, 4><<<grid, 512, lds, stream>>>(a);
+    return hipGetLastError();
+  });
+}
+
+hipError_t launch_adapter_long(const AdapterArgs& a, hipStream_t stream) {
+  const dim3 down(a.splits, (a.max_rows + kDownRows - 1) / kDownRows, a.runs);
+  const dim3 up((a.outs + kUpOuts - 1) / kUpOuts, (a.max_rows + kUpRows - 1) / kUpRows, a.runs);
+  return by_type(a.dtype, [&](auto type) {
+    constexpr uint32_t kType = decltype(type)::value;
+    if (a.max_rank16) adapter_down_kernel<kType><<<down, 256, 0, stream>>>(a);
     adapter_up_kernel<kType><<<up, 256, 0, stream>>>(a);
     return hipGetLastError();
-  };
-  if (a.dtype == kAdapterF32) return go(std::integral_constant<uint32_t, kAdapterF32>{});
-  if (a.dtype == kAdapterF16) return go(std::integral_constant<uint32_t, kAdapterF16>{});
-  return go(std::integral_constant<uint32_t, kAdapterBF16>{});
+  });
 }
 
 }  // namespace jma

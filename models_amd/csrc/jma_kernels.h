@@ -339,6 +339,9 @@ hipError_t launch_paged_table(const PagedTableArgs& a, hipStream_t stream);
 // ---------------------------------------------------------------- low-rank adapters (jma_adapters.hip)
 
 hipError_t launch_adapter_load(const AdapterLoadArgs& a, hipStream_t stream);
-hipError_t launch_adapter_apply(const AdapterArgs& a, hipStream_t stream);
+// Runs of few rows (a.row_block 1, 2 or 4, a.cols * a.row_block at most kFewFloats), in one launch; and
+// runs of any, in two, with scratch.
+hipError_t launch_adapter_few(const AdapterArgs& a, hipStream_t stream);
+hipError_t launch_adapter_long(const AdapterArgs& a, hipStream_t stream);
 
 }  // namespace jma

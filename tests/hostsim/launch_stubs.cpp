@@ -393,22 +393,43 @@ hipError_t launch_adapter_load(const AdapterLoadArgs& a, hipStream_t stream) {
   });
 }
 
-hipError_t launch_adapter_apply(const AdapterArgs& a, hipStream_t stream) {
-  return run(stream, "adapter_kernels", [a] {
-    const uint64_t e = adapter_elem(a.dtype);
-    check_grid(a.splits, (a.max_rows + 7) / 8, a.runs);
-    if (a.runs > kRunsPerLaunch || (uint64_t)a.splits * a.cols_per_split < a.cols) hipsim_fail("launch does not cover the call");
-    for (uint32_t i = 0; i < a.runs; ++i) {
-      const AdapterRun& r = a.run[i];
-      if (r.rows > a.max_rows || r.rank16 > a.max_rank16) hipsim_fail("run past the launch's sizes");
-      check(a.x + (uint64_t)r.row0 * a.cols, (uint64_t)r.rows * a.cols * 4, "input");
-      if (a.base) check(a.base + (uint64_t)r.row0 * a.outs, (uint64_t)r.rows * a.outs * 4, "base");
-      check(a.out + (uint64_t)r.row0 * a.outs, (uint64_t)r.rows * a.outs * 4, "output");
-      if (r.rank16 == 0) continue;
+namespace {
+void check_runs(const AdapterArgs& a, bool scratch) {
+  const uint64_t e = adapter_elem(a.dtype);
+  if (a.runs > kMaxRuns) hipsim_fail("too many runs");
+  for (uint32_t i = 0; i < a.runs; ++i) {
+    const AdapterRun& r = a.run[i];
+    if (r.rows > a.max_rows) hipsim_fail("run past the launch's sizes");
+    check(a.x + (uint64_t)r.row0 * a.cols, (uint64_t)r.rows * a.cols * 4, "input");
+    if (a.base) check(a.base + (uint64_t)r.row0 * a.outs, (uint64_t)r.rows * a.outs * 4, "base");
+    check(a.out + (uint64_t)r.row0 * a.outs, (uint64_t)r.rows * a.outs * 4, "output");
+    if (r.rank16 == 0) continue;
+    if (scratch) {
+      if (r.rank16 > a.max_rank16) hipsim_fail("run of more ranks than the scratch");
       check(a.down + (uint64_t)r.row0 * a.splits * a.max_rank16, (uint64_t)r.rows * a.splits * a.max_rank16 * 4, "products");
-      check((const char*)a.a + r.a_at * e, (uint64_t)r.rank16 * a.cols * e, "stored A");
-      check((const char*)a.b + r.b_at * e, (uint64_t)r.rank16 * a.outs * e, "stored B");
     }
+    check((const char*)a.a + r.a_at * e, (uint64_t)r.rank16 * a.cols * e, "stored A");
+    check((const char*)a.b + r.b_at * e, (uint64_t)r.rank16 * a.outs * e, "stored B");
+  }
+}
+}  // namespace
+
+hipError_t launch_adapter_few(const AdapterArgs& a, hipStream_t stream) {
+  return run(stream, "adapter_few_kernel", [a] {
+    check_grid((a.outs + kFewOuts - 1) / kFewOuts, (a.max_rows + a.row_block - 1) / a.row_block, a.runs);
+    if (a.row_block != 1 && a.row_block != 2 && a.row_block != 4) hipsim_fail("unknown row block");
+    if ((uint64_t)a.row_block * a.cols > kFewFloats) hipsim_fail("rows do not fit the LDS");
+    check_runs(a, false);
+  });
+}
+
+hipError_t launch_adapter_long(const AdapterArgs& a, hipStream_t stream) {
+  return run(stream, "adapter_long_kernels", [a] {
+    check_grid(a.splits, (a.max_rows + kDownRows - 1) / kDownRows, a.runs);
+    check_grid((a.outs + kUpOuts - 1) / kUpOuts, (a.max_rows + kUpRows - 1) / kUpRows, a.runs);
+    if ((uint64_t)a.splits * a.cols_per_split < a.cols || (uint64_t)(a.splits - 1) * a.cols_per_split >= a.cols)
+      hipsim_fail("pieces do not cover the columns");
+    check_runs(a, true);
   });
 }
 
