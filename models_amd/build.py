@@ -2,7 +2,7 @@
 
 Run ``python -m models_amd.build`` or call :func:`build`. The library is the product: the HIP
 kernels (csrc/jma_kernels.hip, csrc/jma_quant.hip, csrc/jma_qgemm.hip, csrc/jma_paged.hip,
-csrc/jma_adapters.hip) and the C-ABI runtime (csrc/jma_runtime.cpp) declared in
+csrc/jma_paged_prefill.hip, csrc/jma_adapters.hip) and the C-ABI runtime (csrc/jma_runtime.cpp) declared in
 include/jmodels_attn.h.
 """
 
@@ -18,7 +18,7 @@ LIB_NAME = "libjmodels_attn.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = [os.path.join(HERE, "csrc", "jma_kernels.hip"), os.path.join(HERE, "csrc", "jma_quant.hip"),
            os.path.join(HERE, "csrc", "jma_qgemm.hip"), os.path.join(HERE, "csrc", "jma_paged.hip"),
-           os.path.join(HERE, "csrc", "jma_adapters.hip"),
+           os.path.join(HERE, "csrc", "jma_paged_prefill.hip"), os.path.join(HERE, "csrc", "jma_adapters.hip"),
            os.path.join(HERE, "csrc", "jma_runtime.cpp")]
 
 HIPCC_FLAGS = [

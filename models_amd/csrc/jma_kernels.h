@@ -334,6 +334,8 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, h
 // max_pages: pages that the row furthest back sees.
 hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, uint32_t max_pages, hipStream_t stream);
 hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, hipStream_t stream);
+// Chunks of many rows over an f16 cache (no selected pages).
+hipError_t launch_paged_prefill(const PagedAttendArgs& a, uint32_t d, hipStream_t stream);
 hipError_t launch_paged_table(const PagedTableArgs& a, hipStream_t stream);
 
 // ---------------------------------------------------------------- low-rank adapters (jma_adapters.hip)

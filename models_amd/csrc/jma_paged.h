@@ -82,8 +82,9 @@ struct PagedAttendArgs {
   const uint32_t* pages; // selected pages [rows][hkv][budget], ascending, kNoPage behind; null: every page
   float scale;           // score scale x log2(e)
   uint32_t num_heads, group, window, budget;
-  uint32_t head_groups;  // ceil(group / 16)
-  uint32_t rows_per_block;  // query rows of one workgroup's 16 columns
+  uint32_t head_groups;  // groups of at most 16 (prefill: 32) query heads of a kv head
+  uint32_t rows_per_block;  // query rows of one workgroup
+  uint32_t rows_per_stripe, heads_per_stripe;  // prefill: query rows and heads of a wave's 32 columns
   uint32_t max_blocks;   // row blocks of the chunk with the most
   uint32_t tiles_per_split, max_splits;
   uint32_t chunks;
@@ -182,6 +183,54 @@ inline PagedPlan plan_paged(PagedChunk* c, uint32_t chunks, uint32_t group, uint
   }
   if (p.max_splits > 1) {
     p.part_bytes = items * kHeadSlots * (d + 4) * 4;
+    p.ticket_bytes = (uint64_t)chunks * p.max_blocks * per * 4;
+  }
+  return p;
+}
+
+// The prefill kernel: waves of a workgroup (32 columns each), storage tiles of a step, and floats of one
+// workgroup's partial state: [wave][d / 8 words of O^T, then (m, l)][64 lanes] float4.
+constexpr int kPrefillWaves = 4;
+JMA_HD constexpr int paged_prefill_tiles(int d) { return d >= 256 ? 1 : 2; }
+JMA_HD constexpr uint32_t paged_prefill_item(int d) { return (uint32_t)(kPrefillWaves * (d / 8 + 1) * 64 * 4); }
+
+// Plan of one prefill launch: blocks are split only where there are too few to fill `target` places, into
+// as many equal parts as fill them, of at least 8 tiles.
+inline PagedPlan plan_paged_prefill(PagedChunk* c, uint32_t chunks, uint32_t rows_per_block, uint32_t head_groups,
+                                    uint32_t hkv, uint32_t d, uint32_t window, uint32_t target) {
+  PagedPlan p;
+  p.rows_per_block = rows_per_block;
+  p.head_groups = head_groups;
+  const uint64_t per = (uint64_t)hkv * head_groups;
+  uint64_t units = 0;
+  uint32_t longest = 1;
+  auto each = [&](uint32_t i, auto&& f) {
+    for (uint32_t r0 = 0; r0 < c[i].rows; r0 += rows_per_block) {
+      uint32_t t0, t1;
+      paged_range(c[i].start + r0, c[i].start + std::min(r0 + rows_per_block, c[i].rows) - 1, window, 0, 0, kTileSlots, t0, t1);
+      f(t1 - t0);
+    }
+  };
+  for (uint32_t i = 0; i < chunks; ++i) {
+    each(i, [&](uint32_t n) { longest = std::max(longest, n); });
+    const uint32_t blocks = (c[i].rows + rows_per_block - 1) / rows_per_block;
+    p.max_blocks = std::max(p.max_blocks, blocks);
+    units += blocks * per;
+  }
+  const uint32_t ways = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(kMaxSplits, target / std::max<uint64_t>(units, 1)));
+  p.tiles_per_split = std::max(8u, (longest + ways - 1) / ways);
+  p.tiles_per_split = (p.tiles_per_split + 1) / 2 * 2;
+  uint64_t items = 0;
+  for (uint32_t i = 0; i < chunks; ++i) {
+    uint32_t most = 1;
+    each(i, [&](uint32_t n) { most = std::max(most, (n + p.tiles_per_split - 1) / p.tiles_per_split); });
+    c[i].nsplit = most;
+    c[i].part0 = (uint32_t)items;
+    if (most > 1) items += (uint64_t)((c[i].rows + rows_per_block - 1) / rows_per_block) * per * most;
+    p.max_splits = std::max(p.max_splits, most);
+  }
+  if (p.max_splits > 1) {
+    p.part_bytes = items * paged_prefill_item((int)d) * 4;
     p.ticket_bytes = (uint64_t)chunks * p.max_blocks * per * 4;
   }
   return p;

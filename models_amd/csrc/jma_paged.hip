@@ -15,30 +15,10 @@
 
 #include <type_traits>
 
-#include "jma_kernels.h"
+#include "jma_paged_device.h"
 
 namespace jma {
 namespace {
-
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef float float4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
-
-#define JMA_INL __attribute__((always_inline))
-
-// Raises an error in the context's error word, in host memory: one byte per kind.
-constexpr int kErrNonFinite = 0, kErrBadPage = 2;
-__device__ __forceinline__ void report(int* err, int kind) {
-  __hip_atomic_store((uint8_t*)err + kind, (uint8_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-}
-
-// x0*c - x1*s and x0*s + x1*c, every product and sum rounded on its own.
-__device__ __forceinline__ void rotate_pair(float& x0, float& x1, float c, float s) {
-#pragma clang fp contract(off)
-  const float y0 = x0 * c - x1 * s, y1 = x0 * s + x1 * c;
-  x0 = y0;
-  x1 = y1;
-}
 
 // ================================================================ append
 
@@ -487,38 +467,6 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
 
 // ================================================================ attention
 
-__device__ __forceinline__ void swap16(float x, float& a, float& b) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  a = __uint_as_float(r[0]);
-  b = __uint_as_float(r[1]);
-}
-__device__ __forceinline__ void swap32(float x, float& a, float& b) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  a = __uint_as_float(r[0]);
-  b = __uint_as_float(r[1]);
-}
-// Over the four 16-lane groups, which hold the same column.
-__device__ __forceinline__ float max_groups(float x) {
-  float a, b;
-  swap16(x, a, b);
-  x = fmaxf(a, b);
-  swap32(x, a, b);
-  return fmaxf(a, b);
-}
-__device__ __forceinline__ float sum_groups(float x) {
-  float a, b;
-  swap16(x, a, b);
-  x = a + b;
-  swap32(x, a, b);
-  return a + b;
-}
-
-// Partial states move between workgroups with 16-byte device-coherent accesses (sc1).
-constexpr int kCoherent = 16;
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_rsrc(float* p) {
-  return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7FFFFFF0, 0x00020000);
-}
-
 // One step's K and V of one lane, in matrix-core operand order (below).
 template <typename KV, int D>
 struct Step;
@@ -562,7 +510,7 @@ struct Step<float, D> {
 // halves far from f16's ends; p is formed as 2^(s - m + 6) for the same reason.
 //
 // Positions a column does not see are masked after the product, and values that are no finite number
-// in a step that is masked in part reach only the columns that see them: 0 x inf is no 0.
+// in a step that is masked in part reach only the columns that see them (0 x inf is no 0), as NaN.
 template <typename KV, int D, bool kSelected>
 __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const PagedAttendArgs a) {
   constexpr bool kF16 = std::is_same<KV, _Float16>::value;
@@ -758,27 +706,32 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
       return o;
     };
     if (!whole) {
-      // Values here that are no finite number: each row's columns take their product with the slots
-      // that the row does not see set to zero.
-      bool odd = false;
+      // Values here that are no finite number are left out of the product, and what they make of the
+      // columns that see them is added: a second product counts, for each output, the ones its column sees.
+      uint32_t odd = 0;
 #pragma unroll
-      for (int n = 0; n < kNv; ++n)
+      for (int n = 0; n < kNv; ++n) odd |= not_finite(x.v[n]);
+      if (__ballot(odd != 0) != 0) {
+        std::conditional_t<kF16, half8_t, float4_t> sees;
 #pragma unroll
-        for (int e = 0; e < kNs; ++e) odd |= !(fabsf((float)x.v[n][e]) < INFINITY);
-      if (__ballot(odd) != 0) {
-        for (uint32_t r = 0; r < rows; ++r) {
-          const uint32_t rp = pos0 + r, rf = first_visible(rp, a.window);
+        for (int e = 0; e < kNs; ++e) {
+          const uint32_t p = p0 + kNs * g + e;
+          sees[e] = p >= cfirst && p <= cpos ? 1.0f : 0.0f;
+        }
 #pragma unroll
-          for (int n = 0; n < kNv; ++n) {
-            auto v = x.v[n];
+        for (int n = 0; n < kNv; ++n) {
+          auto v = x.v[n], is = x.v[n];
+          split_finite(v, is);
+          float4_t count = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (kF16) {
+            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees, count, 0, 0, 0);
+          } else {
 #pragma unroll
-            for (int e = 0; e < kNs; ++e) {
-              const uint32_t p = p0 + kNs * g + e;
-              v[e] = p < rf || p > rp ? (KV)0.0f : v[e];
-            }
-            const float4_t o = product(v, acc[n]);
-            acc[n] = col_row == r ? o : acc[n];
+            for (int e = 0; e < 4; ++e) count = __builtin_amdgcn_mfma_f32_16x16x4f32(is[e], sees[e], count, 0, 0, 0);
           }
+          acc[n] = product(v, acc[n]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][e] = count[e] > 0.0f ? NAN : acc[n][e];
         }
         return;
       }
@@ -841,11 +794,8 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
       finish(c, e, o, L);
     } else {
       const uint32_t at = ((split * 16 + c) * (D + 4) + e) * 4;
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4_t, o), rs, at, 0, kCoherent);
-      if (e == 0) {
-        const float4_t ml = {M, L, 0.f, 0.f};
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4_t, ml), rs, at + D * 4, 0, kCoherent);
-      }
+      store_part(rs, at, o);
+      if (e == 0) store_part(rs, at + D * 4, float4_t{M, L, 0.f, 0.f});
     }
   }
   if (ns == 1) return;
@@ -857,17 +807,14 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
   __syncthreads();
   if (s_ticket + 1 != ns) return;
   if (threadIdx.x == 0) __hip_atomic_store(&a.tickets[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  auto coherent = [&](uint32_t at) JMA_INL {
-    return __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, kCoherent));
-  };
   for (uint32_t k = threadIdx.x; k < cols * (D / 4); k += 64 * kW) {
     const uint32_t c = k / (D / 4), e = 4 * (k % (D / 4));
     float M = -INFINITY, L = 0.0f;
-    for (uint32_t s = 0; s < ns; ++s) M = fmaxf(M, coherent(((s * 16 + c) * (D + 4) + D) * 4)[0]);
+    for (uint32_t s = 0; s < ns; ++s) M = fmaxf(M, load_part(rs, ((s * 16 + c) * (D + 4) + D) * 4)[0]);
     float4_t o = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t s = 0; s < ns; ++s) {
       const uint32_t at = ((s * 16 + c) * (D + 4)) * 4;
-      const float4_t ml = coherent(at + D * 4), x = coherent(at + e * 4);
+      const float4_t ml = load_part(rs, at + D * 4), x = load_part(rs, at + e * 4);
       const float f = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - M);
       L = fmaf(ml[1], f, L);
 #pragma unroll

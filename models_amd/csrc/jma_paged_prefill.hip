@@ -1,0 +1,344 @@
+// gfx950 kernel of the paged KV cache for chunks of many rows:
+//
+//   paged_prefill_kernel   causal attention of a chunk over its sequence's pages, f16 caches
+#include "jma_paged_device.h"
+
+namespace jma {
+namespace {
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+// 16 bytes a lane from global memory straight into LDS (lane i's at lds + 16 i).
+__device__ __forceinline__ void dma16(const _Float16* base, _Float16* lds, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16*>(base), 0, 0x7FFFFFF0, 0x00020000),
+      (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 0);
+}
+
+// Which slot of a tile row i of the score product is (bits 2 and 3 exchanged), and where 16-byte piece c
+// of a 64-byte row r lies in LDS: the eight lanes of one LDS cycle read the same piece of eight rows,
+// which the exchange spreads over all banks.
+__device__ __forceinline__ uint32_t swap23(uint32_t i) { return (i & ~12u) | ((i & 4u) << 1) | ((i & 8u) >> 1); }
+__device__ __forceinline__ uint32_t swz_k(uint32_t slot) { return ((slot >> 1) & 1u) | ((slot >> 2) & 2u); }
+__device__ __forceinline__ uint32_t swz_v(uint32_t row) { return (row >> 1) & 3u; }
+
+// Workgroup = (split, kv head x head group x block of query rows, chunk); each of its four waves owns 32
+// matrix-core columns = (query row, query head) pairs, and all share the K and V tiles, which
+// direct-to-LDS loads bring a step (64 slots; 32 at heads of 256) ahead of their use.
+//
+// v_mfma_f32_32x32x16_f16, lane l, j = l % 32, h = l / 32: A[i][k]: i = j, k = 8h + e; B[k][c]: c = j,
+// k = 8h + e; D[i][c]: c = j, i = 8 (e / 4) + 4h + e % 4. S^T = K Q^T with row i of the product at slot
+// swap23(i) leaves a lane the scores of slots 8h .. 8h+7 and 16 + 8h .. 16 + 8h + 7, in order: they are the
+// B operand of O^T = V^T P as they stand.
+//
+// Precision, masks and values that are no number are paged_attend_kernel's: q and p as two f16 halves,
+// each column's q scaled by a power of two.
+template <int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : 2))) void paged_prefill_kernel(const PagedAttendArgs a) {
+  constexpr int S = kPrefillWaves, T = paged_prefill_tiles(D);
+  constexpr int kKS = D / 16, kNb = D / 32, kTile = 32 * D;
+  constexpr int kLoads = T * (D / 16) / S;  // 1 KB loads a wave makes of a step's K (and of its V)
+  constexpr uint32_t kItem = paged_prefill_item(D);
+  __shared__ __attribute__((aligned(16))) _Float16 lx[2 * T * kTile];  // K tiles, then V tiles
+  __shared__ __attribute__((aligned(16))) _Float16 ly[2 * T * kTile];
+  __shared__ uint32_t s_ticket;
+
+  const PagedChunk ch = a.c[blockIdx.z];
+  const uint32_t hkv = a.kv.hkv, R = a.rows_per_stripe, Gz = a.heads_per_stripe;
+  const uint32_t kvh = blockIdx.y % hkv, rest = blockIdx.y / hkv;
+  const uint32_t hg = rest % a.head_groups, rank = rest / a.head_groups;
+  const uint32_t blocks = (ch.rows + S * R - 1) / (S * R);
+  if (rank >= blocks) return;
+  const uint32_t b_row0 = (blocks - 1 - rank) * S * R;  // the longest ranges first
+  const uint32_t b_row1 = min(b_row0 + S * R, ch.rows) - 1;
+  uint32_t t0, t1;
+  paged_range(ch.start + b_row0, ch.start + b_row1, a.window, 0u, a.kv.page_log2, kTileSlots, t0, t1);
+  const uint32_t ns = (t1 - t0 + a.tiles_per_split - 1) / a.tiles_per_split, split = blockIdx.x;
+  if (split >= ns) return;
+  t0 += split * a.tiles_per_split;
+  t1 = min(t1, t0 + a.tiles_per_split);
+
+  const int lane = threadIdx.x & 63, j = lane & 31, h = lane >> 5;
+  const int s = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t row0 = min(b_row0 + s * R, ch.rows - 1);  // a stripe behind the chunk repeats its last row
+  const bool stripe_ok = b_row0 + s * R < ch.rows;
+  const uint32_t rows = min(R, ch.rows - row0), heads = min(Gz, a.group - hg * Gz);
+  const uint32_t pos0 = ch.start + row0, pos1 = pos0 + rows - 1;
+  const uint32_t first0 = first_visible(pos0, a.window), first1 = first_visible(pos1, a.window);
+  // This lane's column; one past the stripe's (row, head) pairs repeats a valid one and is never stored.
+  const uint32_t col_row = min((uint32_t)j / heads, rows - 1);
+  const bool col_ok = stripe_ok && (uint32_t)j / heads < rows;
+  const uint32_t cpos = pos0 + col_row, cfirst = first_visible(cpos, a.window);
+  const uint64_t qat = (((uint64_t)ch.row0 + row0 + col_row) * a.num_heads + kvh * a.group + hg * Gz + j % heads) * D;
+
+  // The page of tile base + lane of this split.
+  const uint32_t* table = a.kv.table + (uint64_t)ch.seq * a.kv.table_stride;
+  const uint32_t tiles_log2 = a.kv.page_log2 - 5;
+  uint32_t pages_at = t0;
+  uint32_t my_page = table[min(t0 + lane, t1 - 1) >> tiles_log2];
+  // This lane's place in a 1 KB piece: 16 rows of 64 bytes, four 16-byte pieces each.
+  const uint32_t lrow = lane / 4;
+  const uint32_t koff = lrow * 64 + ((lane & 3) ^ swz_k(lrow)) * 16, voff = lrow * 64 + ((lane & 3) ^ swz_v(lrow)) * 16;
+  auto stage = [&](uint32_t t, _Float16* lds) JMA_INL {
+    const _Float16* kt[T];
+    const _Float16* vt[T];
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+      const uint32_t tile = min(t + i, t1 - 1);  // a tile behind the last is loaded again, and not used
+      const uint32_t page = __builtin_amdgcn_readlane(my_page, tile - pages_at);
+      const uint64_t at = paged_base(page, hkv, kvh, a.kv.page_log2, D) + (tile & ((1u << tiles_log2) - 1)) * kTile;
+      kt[i] = (const _Float16*)a.kv.k + at;
+      vt[i] = (const _Float16*)a.kv.v + at;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t u = s + S * i, tile = T == 1 ? 0 : u / (D / 16), c = u % (D / 16);
+      dma16(T == 1 || tile == 0 ? kt[0] : kt[T - 1], lds + 512 * u, koff, 1024 * c);
+      dma16(T == 1 || tile == 0 ? vt[0] : vt[T - 1], lds + T * kTile + 512 * u, voff, 1024 * c);
+    }
+  };
+  stage(t0, lx);
+
+  // Q^T operands and the factor of the column's scores.
+  half8_t qhi[kKS], qlo[kKS];
+  float factor;
+  {
+    const float* q = a.q + qat + 8 * h;
+    float4_t x[kKS][2];
+    float top = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        x[ks][i] = *(const float4_t*)(q + 16 * ks + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[ks][i][e]));
+      }
+    top = max_halves(top);
+    int ex = 0;  // top in [2^(ex-1), 2^ex)
+    if (top > 0.0f && top < INFINITY) ex = __builtin_amdgcn_frexp_expf(top);
+    ex = max(ex, -100);
+    factor = __builtin_amdgcn_ldexpf(a.scale, ex - 14);
+#pragma unroll
+    for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        _Float16 hi, lo;
+        halves(__builtin_amdgcn_ldexpf(x[ks][e / 4][e % 4], 14 - ex), hi, lo);
+        qhi[ks][e] = hi;
+        qlo[ks][e] = lo;
+      }
+  }
+
+  float m = -INFINITY, l = 0.0f;
+  float16_t o[kNb];
+#pragma unroll
+  for (int nb = 0; nb < kNb; ++nb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[nb][e] = 0.0f;
+
+  const uint32_t kr = swap23(j), kswz = swz_k(kr), vswz = swz_v(j);
+  auto tile_step = [&](const _Float16* kt, const _Float16* vt, uint32_t p0) JMA_INL {
+    if (p0 > pos1 || p0 + 31 < first0) return;  // this stripe sees none of it
+    float16_t sc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+    for (int k0 = 0; k0 < kKS; k0 += 4) {
+      constexpr int kB = kKS < 4 ? kKS : 4;
+      half8_t kf[kB];
+#pragma unroll
+      for (int i = 0; i < kB; ++i) {
+        const int ks = k0 + i;
+        kf[i] = *(const half8_t*)(kt + (ks / 2) * 1024 + kr * 32 + 8 * ((2 * (ks % 2) + h) ^ kswz));
+      }
+#pragma unroll
+      for (int i = 0; i < kB; ++i) {
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], qlo[k0 + i], sc, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], qhi[k0 + i], sc, 0, 0, 0);
+      }
+    }
+    const bool whole = p0 + 31 <= pos0 && p0 >= first1;
+    if (!whole) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t p = p0 + 16 * (e / 8) + 8 * h + e % 8;
+        sc[e] = p >= cfirst && p <= cpos ? sc[e] : -INFINITY;
+      }
+    }
+    float tmax = sc[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, sc[e]);
+    tmax = max_halves(tmax) * factor;
+    // The running maximum rises only by more than 2^8: most tiles rescale nothing.
+    const bool up = m == -INFINITY ? tmax > -INFINITY : tmax > m + 8.0f;
+    if (__ballot(up) != 0) {
+      const float mn = up ? tmax : m;
+      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int nb = 0; nb < kNb; ++nb) o[nb] *= alpha;
+    }
+    const float shift = 6.0f - (m == -INFINITY ? 0.0f : m);
+    half8_t ph[2], pl[2];
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const float p0_ = __builtin_amdgcn_exp2f(fmaf(sc[e], factor, shift)), p1_ = __builtin_amdgcn_exp2f(fmaf(sc[e + 1], factor, shift));
+      sum[0] += p0_;
+      sum[1] += p1_;
+      const half2_t hi = __builtin_convertvector((float2_t{p0_, p1_}), half2_t);
+      const half2_t lo = __builtin_convertvector((float2_t{p0_ - (float)hi[0], p1_ - (float)hi[1]}), half2_t);
+      ph[e / 8][e % 8] = hi[0];
+      ph[e / 8][e % 8 + 1] = hi[1];
+      pl[e / 8][e % 8] = lo[0];
+      pl[e / 8][e % 8 + 1] = lo[1];
+    }
+    l += sum[0] + sum[1];
+    auto value = [&](int nb, int b) JMA_INL {
+      return *(const half8_t*)(vt + (32 * nb + j) * 32 + 8 * ((2 * b + h) ^ vswz));
+    };
+    if (!whole) {
+      // Values here that are no finite number are left out of the product, and what they make of the
+      // columns that see them is added: a second product counts, for each output, the ones its column sees.
+      uint32_t odd = 0;
+#pragma unroll
+      for (int nb = 0; nb < kNb; ++nb) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) odd |= not_finite(value(nb, b));
+        asm volatile("" : "+v"(odd)::"memory");  // the products read the values again: kept, they would spill
+      }
+      if (__ballot(odd != 0) != 0) {
+        half8_t sees[2];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t p = p0 + 16 * (e / 8) + 8 * h + e % 8;
+          sees[e / 8][e % 8] = p >= cfirst && p <= cpos ? (_Float16)1.0f : (_Float16)0.0f;
+        }
+#pragma unroll
+        for (int nb = 0; nb < kNb; ++nb) {
+          asm volatile("" ::: "memory");
+          float16_t count;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) count[e] = 0.0f;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            half8_t v = value(nb, b), is;
+            split_finite(v, is);
+            count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees[b], count, 0, 0, 0);
+            o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[b], o[nb], 0, 0, 0);
+            o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[b], o[nb], 0, 0, 0);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[nb][e] = count[e] > 0.0f ? NAN : o[nb][e];
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int nb = 0; nb < kNb; nb += 2) {
+      constexpr int kB = kNb < 2 ? 1 : 2;
+      half8_t v[kB][2];
+#pragma unroll
+      for (int i = 0; i < kB; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) v[i][b] = value(nb + i, b);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+          o[nb + i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][b], pl[b], o[nb + i], 0, 0, 0);
+          o[nb + i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][b], ph[b], o[nb + i], 0, 0, 0);
+        }
+    }
+  };
+
+  // One barrier a step: behind it every wave's loads of this step have landed (each wave waited for its
+  // own) and every wave has done with the array that the next step's loads then overwrite.
+  auto step = [&](uint32_t t, _Float16* lds, _Float16* next) JMA_INL {
+    __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));  // vmcnt(0)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + T < t1) {
+      if (min(t + 2 * T, t1) > pages_at + 64) {  // the next step's pages
+        pages_at = t + T;
+        my_page = table[min(pages_at + lane, t1 - 1) >> tiles_log2];
+      }
+      stage(t + T, next);
+    }
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+      if (t + i < t1) tile_step(lds + i * kTile, lds + (T + i) * kTile, 32 * (t + i));
+  };
+  for (uint32_t t = t0; t < t1; t += 2 * T) {
+    step(t, lx, ly);
+    if (t + T < t1) step(t + T, ly, lx);
+  }
+
+  l = sum_halves(l);
+  auto finish = [&](auto&& chunk_of, float sum) JMA_INL {
+    if (__ballot(col_ok && !(sum > 0.0f && sum < INFINITY)) != 0 && lane == 0) report(a.err, kErrNonFinite);
+    const float inv = sum > 0.0f ? 1.0f / sum : sum;
+    float* out = a.out + qat + 4 * h;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      const float4_t x = chunk_of(c);
+      if (col_ok) *(float4_t*)(out + 8 * c) = x * inv;
+    }
+  };
+  auto mine = [&](int c) JMA_INL {
+    return float4_t{o[c / 4][4 * (c % 4)], o[c / 4][4 * (c % 4) + 1], o[c / 4][4 * (c % 4) + 2], o[c / 4][4 * (c % 4) + 3]};
+  };
+  if (ns == 1) {
+    finish(mine, l);
+    return;
+  }
+  // Split blocks: the states are acknowledged (visible device-wide) before the ticket is taken; the last
+  // workgroup of the block joins them in split order, whichever it is.
+  const uint64_t unit = (uint64_t)blockIdx.z * gridDim.y + blockIdx.y;
+  float* part = a.part + (ch.part0 + (uint64_t)blockIdx.y * ch.nsplit) * kItem;
+  const __amdgpu_buffer_rsrc_t rs = part_rsrc(part);
+  auto word = [&](uint32_t sp, int c) JMA_INL { return (uint32_t)((sp * kItem + ((s * (D / 8 + 1) + c) * 64 + lane) * 4) * 4); };
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) store_part(rs, word(split, c), mine(c));
+  store_part(rs, word(split, D / 8), float4_t{m, l, 0.0f, 0.0f});
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(&a.tickets[unit], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (s_ticket + 1 != ns) return;
+  if (threadIdx.x == 0) __hip_atomic_store(&a.tickets[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  float M = -INFINITY, L = 0.0f;
+  for (uint32_t sp = 0; sp < ns; ++sp) M = fmaxf(M, load_part(rs, word(sp, D / 8))[0]);
+  float4_t y[D / 8];
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) y[c] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t sp = 0; sp < ns; ++sp) {
+    const float4_t ml = load_part(rs, word(sp, D / 8));
+    const float f = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - M);
+    L = fmaf(ml[1], f, L);
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      const float4_t x = load_part(rs, word(sp, c));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[c][e] = fmaf(x[e], f, y[c][e]);
+    }
+  }
+  finish([&](int c) JMA_INL { return y[c]; }, L);
+}
+
+}  // namespace
+
+hipError_t launch_paged_prefill(const PagedAttendArgs& a, uint32_t d, hipStream_t stream) {
+  const dim3 grid(a.max_splits, a.max_blocks * a.kv.hkv * a.head_groups, a.chunks);
+  switch (d) {
+    case 32: paged_prefill_kernel<32><<<grid, 64 * kPrefillWaves, 0, stream>>>(a); break;
+    case 64: paged_prefill_kernel<64><<<grid, 64 * kPrefillWaves, 0, stream>>>(a); break;
+    case 128: paged_prefill_kernel<128><<<grid, 64 * kPrefillWaves, 0, stream>>>(a); break;
+    case 256: paged_prefill_kernel<256><<<grid, 64 * kPrefillWaves, 0, stream>>>(a); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace jma

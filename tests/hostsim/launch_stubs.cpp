@@ -383,6 +383,41 @@ hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, h
   });
 }
 
+hipError_t launch_paged_prefill(const PagedAttendArgs& a, uint32_t d, hipStream_t stream) {
+  return run(stream, "paged_prefill_kernel", [a, d] {
+    const uint64_t units = (uint64_t)a.max_blocks * a.kv.hkv * a.head_groups;
+    check_grid(a.max_splits, units, a.chunks);
+    if (a.pages || a.rows_per_block != kPrefillWaves * a.rows_per_stripe || a.rows_per_stripe * a.heads_per_stripe > 32 ||
+        a.heads_per_stripe * a.head_groups < a.group)
+      hipsim_fail("stripes do not cover the heads");
+    if (a.max_splits > 1) {
+      check(a.tickets, units * a.chunks * 4, "tickets");
+      for (uint64_t i = 0; i < units * a.chunks; ++i)
+        if (a.tickets[i] != 0) hipsim_fail("a ticket is not zero");
+    }
+    for (uint32_t i = 0; i < a.chunks; ++i) {
+      const PagedChunk& c = a.c[i];
+      const uint64_t qd = (uint64_t)a.num_heads * d;
+      check(a.q + c.row0 * qd, c.rows * qd * 4, "q");
+      check(a.out + c.row0 * qd, c.rows * qd * 4, "out");
+      const uint32_t blocks = (c.rows + a.rows_per_block - 1) / a.rows_per_block;
+      if (blocks > a.max_blocks) hipsim_fail("chunk of more blocks than the grid");
+      for (uint32_t b = 0; b < blocks; ++b) {
+        const uint32_t r0 = b * a.rows_per_block, r1 = std::min(r0 + a.rows_per_block, c.rows) - 1;
+        uint32_t t0, t1;
+        paged_range(c.start + r0, c.start + r1, a.window, 0, a.kv.page_log2, kTileSlots, t0, t1);
+        const uint32_t ns = (t1 - t0 + a.tiles_per_split - 1) / a.tiles_per_split;
+        if (ns > c.nsplit || ns > a.max_splits) hipsim_fail("block of more splits than planned");
+      }
+      const uint64_t item = paged_prefill_item((int)d) * 4ull;
+      if (item * c.nsplit > 0x7FFFFFF0u) hipsim_fail("a block's states past 32-bit offsets");
+      if (c.nsplit > 1)
+        check((const char*)a.part + c.part0 * item, (uint64_t)blocks * a.kv.hkv * a.head_groups * c.nsplit * item, "split states");
+      check_pages(a.kv, c.seq, first_visible(c.start, a.window) >> a.kv.page_log2, (c.start + c.rows - 1) >> a.kv.page_log2, d, 2);
+    }
+  });
+}
+
 hipError_t launch_adapter_load(const AdapterLoadArgs& a, hipStream_t stream) {
   return run(stream, "adapter_load_kernel", [a] {
     const uint64_t e = adapter_elem(a.dtype), r16 = adapter_rank16(a.rank);
