@@ -192,6 +192,8 @@ inline PagedPlan plan_paged(PagedChunk* c, uint32_t chunks, uint32_t group, uint
 // workgroup's partial state: [wave][d / 8 words of O^T, then (m, l)][64 lanes] float4.
 constexpr int kPrefillWaves = 4;
 JMA_HD constexpr int paged_prefill_tiles(int d) { return d >= 256 ? 1 : 2; }
+// Waves of one SIMD: what the registers of a wave (q and O^T of 32 columns) leave room for.
+JMA_HD constexpr int paged_prefill_waves_per_simd(int d) { return d >= 256 ? 1 : d >= 128 ? 2 : d >= 64 ? 3 : 4; }
 JMA_HD constexpr uint32_t paged_prefill_item(int d) { return (uint32_t)(kPrefillWaves * (d / 8 + 1) * 64 * 4); }
 
 // Plan of one prefill launch: blocks are split only where there are too few to fill `target` places, into

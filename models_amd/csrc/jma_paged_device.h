@@ -84,6 +84,18 @@ __device__ __forceinline__ void halves(float x, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(x - (float)hi);
 }
 
+// x minus the low (high) half of h, in one instruction.
+__device__ __forceinline__ float minus_low(float x, half2_t h) {
+  float y;
+  asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(h), "v"(x));
+  return y;
+}
+__device__ __forceinline__ float minus_high(float x, half2_t h) {
+  float y;
+  asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(h), "v"(x));
+  return y;
+}
+
 // Nonzero where one of the halves is infinite or no number.
 __device__ __forceinline__ uint32_t not_finite(const half8_t& x) {
   const uint4_t w = __builtin_bit_cast(uint4_t, x);

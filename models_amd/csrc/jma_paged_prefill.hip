@@ -34,7 +34,7 @@ __device__ __forceinline__ uint32_t swz_v(uint32_t row) { return (row >> 1) & 3u
 // Precision, masks and values that are no number are paged_attend_kernel's: q and p as two f16 halves,
 // each column's q scaled by a power of two.
 template <int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : 2))) void paged_prefill_kernel(const PagedAttendArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefill_waves_per_simd(D)))) void paged_prefill_kernel(const PagedAttendArgs a) {
   constexpr int S = kPrefillWaves, T = paged_prefill_tiles(D);
   constexpr int kKS = D / 16, kNb = D / 32, kTile = 32 * D;
   constexpr int kLoads = T * (D / 16) / S;  // 1 KB loads a wave makes of a step's K (and of its V)
@@ -138,8 +138,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 
     for (int e = 0; e < 16; ++e) o[nb][e] = 0.0f;
 
   const uint32_t kr = swap23(j), kswz = swz_k(kr), vswz = swz_v(j);
-  auto tile_step = [&](const _Float16* kt, const _Float16* vt, uint32_t p0) JMA_INL {
-    if (p0 > pos1 || p0 + 31 < first0) return;  // this stripe sees none of it
+  // One tile, in LDS, or (kRobust) in global memory. kMasked: some column of the workgroup may not see all
+  // of it.
+  auto tile_step = [&](const _Float16* kt, const _Float16* vt, uint32_t p0, auto masked, auto robust) JMA_INL {
+    constexpr bool kMasked = decltype(masked)::value, kRobust = decltype(robust)::value;
+    if (kMasked && (p0 > pos1 || p0 + 31 < first0)) return;  // this stripe sees none of it
     float16_t sc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 
 #pragma unroll
       for (int i = 0; i < kB; ++i) {
         const int ks = k0 + i;
-        kf[i] = *(const half8_t*)(kt + (ks / 2) * 1024 + kr * 32 + 8 * ((2 * (ks % 2) + h) ^ kswz));
+        kf[i] = *(const half8_t*)(kt + (ks / 2) * 1024 + kr * 32 + 8 * ((2 * (ks % 2) + h) ^ (kRobust ? 0u : kswz)));
       }
 #pragma unroll
       for (int i = 0; i < kB; ++i) {
@@ -158,8 +161,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 
         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], qhi[k0 + i], sc, 0, 0, 0);
       }
     }
-    const bool whole = p0 + 31 <= pos0 && p0 >= first1;
-    if (!whole) {
+    const bool whole = !kMasked || (p0 + 31 <= pos0 && p0 >= first1);
+    if (kMasked && !whole) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const uint32_t p = p0 + 16 * (e / 8) + 8 * h + e % 8;
@@ -189,7 +192,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 
       sum[0] += p0_;
       sum[1] += p1_;
       const half2_t hi = __builtin_convertvector((float2_t{p0_, p1_}), half2_t);
-      const half2_t lo = __builtin_convertvector((float2_t{p0_ - (float)hi[0], p1_ - (float)hi[1]}), half2_t);
+      const half2_t lo = __builtin_convertvector((float2_t{minus_low(p0_, hi), minus_high(p1_, hi)}), half2_t);
       ph[e / 8][e % 8] = hi[0];
       ph[e / 8][e % 8 + 1] = hi[1];
       pl[e / 8][e % 8] = lo[0];
@@ -197,44 +200,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 
     }
     l += sum[0] + sum[1];
     auto value = [&](int nb, int b) JMA_INL {
-      return *(const half8_t*)(vt + (32 * nb + j) * 32 + 8 * ((2 * b + h) ^ vswz));
+      return *(const half8_t*)(vt + (32 * nb + j) * 32 + 8 * ((2 * b + h) ^ (kRobust ? 0u : vswz)));
     };
-    if (!whole) {
-      // Values here that are no finite number are left out of the product, and what they make of the
-      // columns that see them is added: a second product counts, for each output, the ones its column sees.
-      uint32_t odd = 0;
+    if constexpr (kRobust) {
+      // Values that are no finite number are left out of the product, and what they make of the columns
+      // that see them is added: a second product counts, for each output, the ones its column sees.
+      half8_t sees[2];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t p = p0 + 16 * (e / 8) + 8 * h + e % 8;
+        sees[e / 8][e % 8] = p >= cfirst && p <= cpos ? (_Float16)1.0f : (_Float16)0.0f;
+      }
 #pragma unroll
       for (int nb = 0; nb < kNb; ++nb) {
+        float16_t count;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) odd |= not_finite(value(nb, b));
-        asm volatile("" : "+v"(odd)::"memory");  // the products read the values again: kept, they would spill
-      }
-      if (__ballot(odd != 0) != 0) {
-        half8_t sees[2];
+        for (int e = 0; e < 16; ++e) count[e] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t p = p0 + 16 * (e / 8) + 8 * h + e % 8;
-          sees[e / 8][e % 8] = p >= cfirst && p <= cpos ? (_Float16)1.0f : (_Float16)0.0f;
+        for (int b = 0; b < 2; ++b) {
+          half8_t v = value(nb, b), is;
+          split_finite(v, is);
+          count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees[b], count, 0, 0, 0);
+          o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[b], o[nb], 0, 0, 0);
+          o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[b], o[nb], 0, 0, 0);
         }
 #pragma unroll
-        for (int nb = 0; nb < kNb; ++nb) {
-          asm volatile("" ::: "memory");
-          float16_t count;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) count[e] = 0.0f;
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            half8_t v = value(nb, b), is;
-            split_finite(v, is);
-            count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees[b], count, 0, 0, 0);
-            o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[b], o[nb], 0, 0, 0);
-            o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[b], o[nb], 0, 0, 0);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[nb][e] = count[e] > 0.0f ? NAN : o[nb][e];
-        }
-        return;
+        for (int e = 0; e < 16; ++e) o[nb][e] = count[e] > 0.0f ? NAN : o[nb][e];
       }
+      return;
     }
 #pragma unroll
     for (int nb = 0; nb < kNb; nb += 2) {
@@ -256,7 +249,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 
 
   // One barrier a step: behind it every wave's loads of this step have landed (each wave waited for its
   // own) and every wave has done with the array that the next step's loads then overwrite.
-  auto step = [&](uint32_t t, _Float16* lds, _Float16* next) JMA_INL {
+  auto step = [&](uint32_t t, _Float16* lds, _Float16* next, auto masked) JMA_INL {
     __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));  // vmcnt(0)
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (t + T < t1) {
@@ -266,13 +259,49 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 
       }
       stage(t + T, next);
     }
+    if constexpr (decltype(masked)::value) {
+#pragma unroll 1
+      for (int i = 0; i < T; ++i)
+        if (t + i < t1) tile_step(lds + i * kTile, lds + (T + i) * kTile, 32 * (t + i), masked, std::false_type{});
+    } else {
 #pragma unroll
-    for (int i = 0; i < T; ++i)
-      if (t + i < t1) tile_step(lds + i * kTile, lds + (T + i) * kTile, 32 * (t + i));
+      for (int i = 0; i < T; ++i) tile_step(lds + i * kTile, lds + (T + i) * kTile, 32 * (t + i), masked, std::false_type{});
+    }
   };
+  // Steps whose tiles every column of the workgroup sees whole run in a loop of their own, two at a time.
+  const uint32_t whole0 = (first_visible(ch.start + b_row1, a.window) + 31) / 32, whole1 = (ch.start + b_row0 + 1) / 32;
+  auto fast = [&](uint32_t t) JMA_INL { return t >= whole0 && t + 2 * T <= min(whole1, t1); };
   for (uint32_t t = t0; t < t1; t += 2 * T) {
-    step(t, lx, ly);
-    if (t + T < t1) step(t + T, ly, lx);
+    for (; fast(t); t += 2 * T) {
+      step(t, lx, ly, std::false_type{});
+      step(t + T, ly, lx, std::false_type{});
+    }
+    if (t >= t1) break;
+    step(t, lx, ly, std::true_type{});
+    if (t + T < t1) step(t + T, ly, lx, std::true_type{});
+  }
+
+  // A value that is no finite number, in a tile that a column sees in part, reaches all of the wave's columns
+  // (0 x inf is no 0). A wave with such an output does its tiles again, straight from global memory, and
+  // keeps what it finds then.
+  float odd = 0.0f;
+#pragma unroll
+  for (int nb = 0; nb < kNb; ++nb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) odd = fmaf(o[nb][e], 0.0f, odd);
+  if (__ballot(odd != 0.0f) != 0) {
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int nb = 0; nb < kNb; ++nb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[nb][e] = 0.0f;
+#pragma unroll 1
+    for (uint32_t t = t0; t < t1; ++t) {
+      const uint32_t page = __builtin_amdgcn_readfirstlane(table[t >> tiles_log2]);
+      const uint64_t at = paged_base(page, hkv, kvh, a.kv.page_log2, D) + (t & ((1u << tiles_log2) - 1)) * kTile;
+      tile_step((const _Float16*)a.kv.k + at, (const _Float16*)a.kv.v + at, 32 * t, std::true_type{}, std::true_type{});
+    }
   }
 
   l = sum_halves(l);
