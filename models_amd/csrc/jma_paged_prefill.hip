@@ -138,27 +138,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefi
     for (int e = 0; e < 16; ++e) o[nb][e] = 0.0f;
 
   const uint32_t kr = swap23(j), kswz = swz_k(kr), vswz = swz_v(j);
-  // One tile, in LDS, or (kRobust) in global memory. kMasked: some column of the workgroup may not see all
-  // of it.
-  auto tile_step = [&](const _Float16* kt, const _Float16* vt, uint32_t p0, auto masked, auto robust) JMA_INL {
+  // kN tiles at once, in LDS, or (kRobust) in global memory. kMasked: some column of the workgroup may not
+  // see all of them.
+  auto tile_step = [&](const _Float16* kt, const _Float16* vt, uint32_t p0, auto count, auto masked, auto robust) JMA_INL {
+    constexpr int kN = decltype(count)::value;
     constexpr bool kMasked = decltype(masked)::value, kRobust = decltype(robust)::value;
+    static_assert(kN == 1 || !kMasked, "masked tiles one at a time");
     if (kMasked && (p0 > pos1 || p0 + 31 < first0)) return;  // this stripe sees none of it
-    float16_t sc;
+    float16_t sc[kN];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+    for (int i = 0; i < kN; ++i)
 #pragma unroll
-    for (int k0 = 0; k0 < kKS; k0 += 4) {
-      constexpr int kB = kKS < 4 ? kKS : 4;
-      half8_t kf[kB];
+      for (int e = 0; e < 16; ++e) sc[i][e] = 0.0f;
+    constexpr int kB = kKS * kN < 4 ? kKS : 4 / kN;  // operand reads issued ahead of their products
+#pragma unroll
+    for (int k0 = 0; k0 < kKS; k0 += kB) {
+      half8_t kf[kB][kN];
+#pragma unroll
+      for (int i = 0; i < kB; ++i)
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          const int ks = k0 + i;
+          kf[i][n] = *(const half8_t*)(kt + n * kTile + (ks / 2) * 1024 + kr * 32 + 8 * ((2 * (ks % 2) + h) ^ (kRobust ? 0u : kswz)));
+        }
 #pragma unroll
       for (int i = 0; i < kB; ++i) {
-        const int ks = k0 + i;
-        kf[i] = *(const half8_t*)(kt + (ks / 2) * 1024 + kr * 32 + 8 * ((2 * (ks % 2) + h) ^ (kRobust ? 0u : kswz)));
-      }
 #pragma unroll
-      for (int i = 0; i < kB; ++i) {
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], qlo[k0 + i], sc, 0, 0, 0);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], qhi[k0 + i], sc, 0, 0, 0);
+        for (int n = 0; n < kN; ++n) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i][n], qlo[k0 + i], sc[n], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i][n], qhi[k0 + i], sc[n], 0, 0, 0);
       }
     }
     const bool whole = !kMasked || (p0 + 31 <= pos0 && p0 >= first1);
@@ -166,12 +174,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefi
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const uint32_t p = p0 + 16 * (e / 8) + 8 * h + e % 8;
-        sc[e] = p >= cfirst && p <= cpos ? sc[e] : -INFINITY;
+        sc[0][e] = p >= cfirst && p <= cpos ? sc[0][e] : -INFINITY;
       }
     }
-    float tmax = sc[0];
+    float tmax = sc[0][0];
 #pragma unroll
-    for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, sc[e]);
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, sc[n][e]);
     tmax = max_halves(tmax) * factor;
     // The running maximum rises only by more than 2^8: most tiles rescale nothing.
     const bool up = m == -INFINITY ? tmax > -INFINITY : tmax > m + 8.0f;
@@ -184,23 +194,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefi
       for (int nb = 0; nb < kNb; ++nb) o[nb] *= alpha;
     }
     const float shift = 6.0f - (m == -INFINITY ? 0.0f : m);
-    half8_t ph[2], pl[2];
+    half8_t ph[kN][2], pl[kN][2];
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const float p0_ = __builtin_amdgcn_exp2f(fmaf(sc[e], factor, shift)), p1_ = __builtin_amdgcn_exp2f(fmaf(sc[e + 1], factor, shift));
-      sum[0] += p0_;
-      sum[1] += p1_;
-      const half2_t hi = __builtin_convertvector((float2_t{p0_, p1_}), half2_t);
-      const half2_t lo = __builtin_convertvector((float2_t{minus_low(p0_, hi), minus_high(p1_, hi)}), half2_t);
-      ph[e / 8][e % 8] = hi[0];
-      ph[e / 8][e % 8 + 1] = hi[1];
-      pl[e / 8][e % 8] = lo[0];
-      pl[e / 8][e % 8 + 1] = lo[1];
-    }
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float x0 = __builtin_amdgcn_exp2f(fmaf(sc[n][e], factor, shift)), x1 = __builtin_amdgcn_exp2f(fmaf(sc[n][e + 1], factor, shift));
+        sum[0] += x0;
+        sum[1] += x1;
+        const half2_t hi = __builtin_convertvector((float2_t{x0, x1}), half2_t);
+        const half2_t lo = __builtin_convertvector((float2_t{minus_low(x0, hi), minus_high(x1, hi)}), half2_t);
+        ph[n][e / 8][e % 8] = hi[0];
+        ph[n][e / 8][e % 8 + 1] = hi[1];
+        pl[n][e / 8][e % 8] = lo[0];
+        pl[n][e / 8][e % 8 + 1] = lo[1];
+      }
     l += sum[0] + sum[1];
-    auto value = [&](int nb, int b) JMA_INL {
-      return *(const half8_t*)(vt + (32 * nb + j) * 32 + 8 * ((2 * b + h) ^ (kRobust ? 0u : vswz)));
+    auto value = [&](int n, int nb, int b) JMA_INL {
+      return *(const half8_t*)(vt + n * kTile + (32 * nb + j) * 32 + 8 * ((2 * b + h) ^ (kRobust ? 0u : vswz)));
     };
     if constexpr (kRobust) {
       // Values that are no finite number are left out of the product, and what they make of the columns
@@ -213,39 +225,42 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefi
       }
 #pragma unroll
       for (int nb = 0; nb < kNb; ++nb) {
-        float16_t count;
+        float16_t found;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) count[e] = 0.0f;
+        for (int e = 0; e < 16; ++e) found[e] = 0.0f;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          half8_t v = value(nb, b), is;
+          half8_t v = value(0, nb, b), is;
           split_finite(v, is);
-          count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees[b], count, 0, 0, 0);
-          o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[b], o[nb], 0, 0, 0);
-          o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[b], o[nb], 0, 0, 0);
+          found = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees[b], found, 0, 0, 0);
+          o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[0][b], o[nb], 0, 0, 0);
+          o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[0][b], o[nb], 0, 0, 0);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[nb][e] = count[e] > 0.0f ? NAN : o[nb][e];
+        for (int e = 0; e < 16; ++e) o[nb][e] = found[e] > 0.0f ? NAN : o[nb][e];
       }
       return;
     }
 #pragma unroll
-    for (int nb = 0; nb < kNb; nb += 2) {
-      constexpr int kB = kNb < 2 ? 1 : 2;
-      half8_t v[kB][2];
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int i = 0; i < kB; ++i)
+      for (int nb = 0; nb < kNb; nb += 2) {
+        constexpr int kV = kNb < 2 ? 1 : 2;
+        half8_t v[kV][2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) v[i][b] = value(nb + i, b);
+        for (int i = 0; i < kV; ++i)
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+          for (int b = 0; b < 2; ++b) v[i][b] = value(n, nb + i, b);
 #pragma unroll
-        for (int i = 0; i < kB; ++i) {
-          o[nb + i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][b], pl[b], o[nb + i], 0, 0, 0);
-          o[nb + i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][b], ph[b], o[nb + i], 0, 0, 0);
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int i = 0; i < kV; ++i) o[nb + i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][b], pl[n][b], o[nb + i], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < kV; ++i) o[nb + i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][b], ph[n][b], o[nb + i], 0, 0, 0);
         }
-    }
+      }
   };
+  constexpr std::integral_constant<int, 1> kOne{};
 
   // One barrier a step: behind it every wave's loads of this step have landed (each wave waited for its
   // own) and every wave has done with the array that the next step's loads then overwrite.
@@ -262,10 +277,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefi
     if constexpr (decltype(masked)::value) {
 #pragma unroll 1
       for (int i = 0; i < T; ++i)
-        if (t + i < t1) tile_step(lds + i * kTile, lds + (T + i) * kTile, 32 * (t + i), masked, std::false_type{});
+        if (t + i < t1) tile_step(lds + i * kTile, lds + (T + i) * kTile, 32 * (t + i), kOne, masked, std::false_type{});
     } else {
-#pragma unroll
-      for (int i = 0; i < T; ++i) tile_step(lds + i * kTile, lds + (T + i) * kTile, 32 * (t + i), masked, std::false_type{});
+      tile_step(lds, lds + T * kTile, 32 * t, std::integral_constant<int, T>{}, masked, std::false_type{});
     }
   };
   // Steps whose tiles every column of the workgroup sees whole run in a loop of their own, two at a time.
@@ -300,7 +314,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefi
     for (uint32_t t = t0; t < t1; ++t) {
       const uint32_t page = __builtin_amdgcn_readfirstlane(table[t >> tiles_log2]);
       const uint64_t at = paged_base(page, hkv, kvh, a.kv.page_log2, D) + (t & ((1u << tiles_log2) - 1)) * kTile;
-      tile_step((const _Float16*)a.kv.k + at, (const _Float16*)a.kv.v + at, 32 * t, std::true_type{}, std::true_type{});
+      tile_step((const _Float16*)a.kv.k + at, (const _Float16*)a.kv.v + at, 32 * t, kOne, std::true_type{}, std::true_type{});
     }
   }
 
