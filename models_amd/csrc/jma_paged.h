@@ -233,7 +233,6 @@ inline PagedPlan plan_paged_prefill(PagedChunk* c, uint32_t chunks, uint32_t row
   }
   if (p.max_splits > 1) {
     p.part_bytes = items * paged_prefill_item((int)d) * 4;
-    p.ticket_bytes = (uint64_t)chunks * p.max_blocks * per * 4;
   }
   return p;
 }

@@ -807,18 +807,32 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
   __syncthreads();
   if (s_ticket + 1 != ns) return;
   if (threadIdx.x == 0) __hip_atomic_store(&a.tickets[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // Two round trips: every split's (m, l), and its share of O, eight splits' words in flight.
+  float (*s_all)[16][2] = (float (*)[16][2])s_acc;  // [split][column]
+  for (uint32_t k = threadIdx.x; k < ns * 16; k += 64 * kW) {
+    const float4_t ml = load_part(rs, ((k / 16 * 16 + min(k % 16, cols - 1)) * (D + 4) + D) * 4);
+    s_all[k / 16][k % 16][0] = ml[0];
+    s_all[k / 16][k % 16][1] = ml[1];
+  }
+  __syncthreads();
   for (uint32_t k = threadIdx.x; k < cols * (D / 4); k += 64 * kW) {
     const uint32_t c = k / (D / 4), e = 4 * (k % (D / 4));
     float M = -INFINITY, L = 0.0f;
-    for (uint32_t s = 0; s < ns; ++s) M = fmaxf(M, load_part(rs, ((s * 16 + c) * (D + 4) + D) * 4)[0]);
     float4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t s = 0; s < ns; ++s) {
-      const uint32_t at = ((s * 16 + c) * (D + 4)) * 4;
-      const float4_t ml = load_part(rs, at + D * 4), x = load_part(rs, at + e * 4);
-      const float f = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - M);
-      L = fmaf(ml[1], f, L);
+    for (uint32_t s0 = 0; s0 < ns; s0 += 8) {
+      float4_t x[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], f, o[j]);
+      for (uint32_t i = 0; i < 8; ++i) x[i] = load_part(rs, ((min(s0 + i, ns - 1) * 16 + c) * (D + 4) + e) * 4);
+      if (s0 == 0)
+        for (uint32_t s = 0; s < ns; ++s) M = fmaxf(M, s_all[s][c][0]);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        if (s0 + i >= ns) break;
+        const float ms = s_all[s0 + i][c][0], f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
+        L = fmaf(s_all[s0 + i][c][1], f, L);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(x[i][j], f, o[j]);
+      }
     }
     finish(c, e, o, L);
   }

@@ -1,6 +1,7 @@
 // gfx950 kernel of the paged KV cache for chunks of many rows:
 //
-//   paged_prefill_kernel   causal attention of a chunk over its sequence's pages, f16 caches
+//   paged_prefill_kernel        causal attention of a chunk over its sequence's pages, f16 caches
+//   paged_prefill_join_kernel   the states of row blocks whose range of positions is split
 #include "jma_paged_device.h"
 
 namespace jma {
@@ -41,7 +42,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefi
   constexpr uint32_t kItem = paged_prefill_item(D);
   __shared__ __attribute__((aligned(16))) _Float16 lx[2 * T * kTile];  // K tiles, then V tiles
   __shared__ __attribute__((aligned(16))) _Float16 ly[2 * T * kTile];
-  __shared__ uint32_t s_ticket;
 
   const PagedChunk ch = a.c[blockIdx.z];
   const uint32_t hkv = a.kv.hkv, R = a.rows_per_stripe, Gz = a.heads_per_stripe;
@@ -336,49 +336,86 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(paged_prefi
     finish(mine, l);
     return;
   }
-  // Split blocks: the states are acknowledged (visible device-wide) before the ticket is taken; the last
-  // workgroup of the block joins them in split order, whichever it is.
-  const uint64_t unit = (uint64_t)blockIdx.z * gridDim.y + blockIdx.y;
-  float* part = a.part + (ch.part0 + (uint64_t)blockIdx.y * ch.nsplit) * kItem;
-  const __amdgpu_buffer_rsrc_t rs = part_rsrc(part);
-  auto word = [&](uint32_t sp, int c) JMA_INL { return (uint32_t)((sp * kItem + ((s * (D / 8 + 1) + c) * 64 + lane) * 4) * 4); };
+  // A split block's state, for paged_prefill_join_kernel.
+  float4_t* part = (float4_t*)(a.part + (ch.part0 + (uint64_t)blockIdx.y * ch.nsplit + split) * kItem) + s * (D / 8 + 1) * 64 + lane;
 #pragma unroll
-  for (int c = 0; c < D / 8; ++c) store_part(rs, word(split, c), mine(c));
-  store_part(rs, word(split, D / 8), float4_t{m, l, 0.0f, 0.0f});
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(&a.tickets[unit], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (s_ticket + 1 != ns) return;
-  if (threadIdx.x == 0) __hip_atomic_store(&a.tickets[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  float M = -INFINITY, L = 0.0f;
-  for (uint32_t sp = 0; sp < ns; ++sp) M = fmaxf(M, load_part(rs, word(sp, D / 8))[0]);
-  float4_t y[D / 8];
+  for (int c = 0; c < D / 8; ++c) part[64 * c] = mine(c);
+  part[64 * (D / 8)] = float4_t{m, l, 0.0f, 0.0f};
+}
+
+// Joins the states of split blocks, in split order: workgroup = (four (wave, word of O^T) pairs, block,
+// chunk), one word a thread. A launch of its own: a last workgroup that waited for the
+// others' states and joined them alone took up to 29 us (1000 rows of 4 + 1 heads of 256).
+template <int D>
+__global__ __launch_bounds__(256) void paged_prefill_join_kernel(const PagedAttendArgs a) {
+  constexpr int S = kPrefillWaves;
+  constexpr uint32_t kItem = paged_prefill_item(D);
+  const PagedChunk ch = a.c[blockIdx.z];
+  const uint32_t hkv = a.kv.hkv, R = a.rows_per_stripe, Gz = a.heads_per_stripe;
+  const uint32_t kvh = blockIdx.y % hkv, rest = blockIdx.y / hkv;
+  const uint32_t hg = rest % a.head_groups, rank = rest / a.head_groups;
+  const uint32_t blocks = (ch.rows + S * R - 1) / (S * R);
+  if (rank >= blocks) return;
+  const uint32_t b_row0 = (blocks - 1 - rank) * S * R, b_row1 = min(b_row0 + S * R, ch.rows) - 1;
+  uint32_t t0, t1;
+  paged_range(ch.start + b_row0, ch.start + b_row1, a.window, 0u, a.kv.page_log2, kTileSlots, t0, t1);
+  const uint32_t ns = (t1 - t0 + a.tiles_per_split - 1) / a.tiles_per_split;
+  if (ns == 1) return;
+  const uint32_t lane = threadIdx.x & 63, unit = blockIdx.x * 4 + threadIdx.x / 64;  // (stripe, word)
+  const uint32_t s = unit / (D / 8), c = unit % (D / 8), j = lane & 31, h = lane >> 5;
+  const uint32_t row0 = b_row0 + s * R, heads = min(Gz, a.group - hg * Gz);
+  if (row0 >= ch.rows || j / heads >= min(R, ch.rows - row0)) return;
+  const float4_t* part = (const float4_t*)(a.part + (ch.part0 + (uint64_t)blockIdx.y * ch.nsplit) * kItem) + s * (D / 8 + 1) * 64 + lane;
+  float m = -INFINITY, l = 0.0f;
+  float4_t y = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t sp0 = 0; sp0 < ns; sp0 += 4) {  // four splits' words in flight
+    float4_t ml[4], x[4];
 #pragma unroll
-  for (int c = 0; c < D / 8; ++c) y[c] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t sp = 0; sp < ns; ++sp) {
-    const float4_t ml = load_part(rs, word(sp, D / 8));
-    const float f = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - M);
-    L = fmaf(ml[1], f, L);
+    for (uint32_t i = 0; i < 4; ++i) {
+      const float4_t* p = part + (uint64_t)min(sp0 + i, ns - 1) * (kItem / 4);
+      ml[i] = p[64 * (D / 8)];
+      x[i] = p[64 * c];
+    }
+    float top = m;
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      const float4_t x = load_part(rs, word(sp, c));
+    for (uint32_t i = 0; i < 4; ++i) {
+      if (sp0 + i >= ns) ml[i] = float4_t{-INFINITY, 0.0f, 0.0f, 0.0f};
+      top = fmaxf(top, ml[i][0]);
+    }
+    const float back = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    l *= back;
+    y *= back;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[c][e] = fmaf(x[e], f, y[c][e]);
+    for (uint32_t i = 0; i < 4; ++i) {
+      if (ml[i][0] == -INFINITY) continue;  // it saw nothing
+      const float f = __builtin_amdgcn_exp2f(ml[i][0] - m);
+      l = fmaf(ml[i][1], f, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fmaf(x[i][e], f, y[e]);
     }
   }
-  finish([&](int c) JMA_INL { return y[c]; }, L);
+  if (c == 0 && !(l > 0.0f && l < INFINITY)) report(a.err, kErrNonFinite);
+  const uint64_t at = (((uint64_t)ch.row0 + row0 + j / heads) * a.num_heads + kvh * a.group + hg * Gz + j % heads) * D;
+  *(float4_t*)(a.out + at + 8 * c + 4 * h) = y * (l > 0.0f ? 1.0f / l : l);
+}
+
+template <int D>
+void launch_prefill(const PagedAttendArgs& a, hipStream_t stream) {
+  const uint32_t units = a.max_blocks * a.kv.hkv * a.head_groups;
+  paged_prefill_kernel<D><<<dim3(a.max_splits, units, a.chunks), 64 * kPrefillWaves, 0, stream>>>(a);
+  if (a.max_splits > 1)
+    paged_prefill_join_kernel<D><<<dim3(kPrefillWaves * (D / 8) / 4, units, a.chunks), 256, 0, stream>>>(a);
 }
 
 }  // namespace
 
 hipError_t launch_paged_prefill(const PagedAttendArgs& a, uint32_t d, hipStream_t stream) {
-  const dim3 grid(a.max_splits, a.max_blocks * a.kv.hkv * a.head_groups, a.chunks);
   switch (d) {
-    case 32: paged_prefill_kernel<32><<<grid, 64 * kPrefillWaves, 0, stream>>>(a); break;
-    case 64: paged_prefill_kernel<64><<<grid, 64 * kPrefillWaves, 0, stream>>>(a); break;
-    case 128: paged_prefill_kernel<128><<<grid, 64 * kPrefillWaves, 0, stream>>>(a); break;
-    case 256: paged_prefill_kernel<256><<<grid, 64 * kPrefillWaves, 0, stream>>>(a); break;
+    case 32: launch_prefill<32>(a, stream); break;
+    case 64: launch_prefill<64>(a, stream); break;
+    case 128: launch_prefill<128>(a, stream); break;
+    case 256: launch_prefill<256>(a, stream); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
