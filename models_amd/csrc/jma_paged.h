@@ -53,19 +53,25 @@ struct PagedChunk {
   uint32_t seq, start, rows, row0, nsplit, part0;
 };
 
+// What new rows are made with: QK-norm, then RoPE.
+struct PagedRotation {
+  const float* cos_t;  // [max_positions][pairs]; null: no RoPE
+  const float* sin_t;
+  const float* q_norm_w;  // [d]; null: no norm of that side
+  const float* k_norm_w;
+  float norm_eps;
+  uint32_t v_norm;  // 1: values are normalised without a weight
+  uint32_t pairs, neox;
+};
+
 struct PagedAppendArgs {
   PagedView kv;
   const float* q;  // [rows][num_heads * d]; null: no query is rotated
   const float* k;  // [rows][hkv * d]
   const float* v;
   float* q_out;
-  const float* cos_t;  // [max_positions][pairs]; null: no RoPE
-  const float* sin_t;
-  const float* q_norm_w;
-  const float* k_norm_w;
-  float norm_eps;
-  uint32_t v_norm;
-  uint32_t pairs, neox, num_heads;
+  PagedRotation rot;
+  uint32_t num_heads;
   uint32_t max_tiles;  // storage tiles of the chunk with the most (the grid's x)
   uint32_t max_pages;  // pages of the chunk with the most (the bounds kernel's x)
   uint32_t chunks;
@@ -74,8 +80,11 @@ struct PagedAppendArgs {
 
 struct PagedAttendArgs {
   PagedView kv;
-  const float* q;        // [rows][num_heads * d], rotated
+  const float* q;        // [rows][num_heads * d], rotated, or raw with k_new
   float* out;            // [rows][num_heads * d]
+  const float* k_new;    // chunks of one row: raw keys and values [rows][hkv * d] that the launch appends; null:
+  const float* v_new;    // the rows are appended already
+  PagedRotation rot;
   int* err;
   float* part;           // [item][16][d + 4] partial states (acc, m, l) of split blocks
   uint32_t* tickets;     // [unit], zero between launches
@@ -98,7 +107,9 @@ constexpr uint32_t kSelectPages = 64;
 
 struct PagedSelectArgs {
   PagedView kv;
-  const float* q;      // rotated
+  const float* q;      // rotated, or raw with `raw`
+  PagedRotation rot;
+  uint32_t raw;
   uint32_t* pages;     // out: [rows][hkv][budget]
   uint64_t* keys;      // scratch [row slot][hkv][key_stride]: the pages' scores as ordered integers
   uint32_t* tickets;   // [row slot][hkv], zero between launches
@@ -117,6 +128,9 @@ struct PagedTableArgs {
   uint32_t at[kTableWrites], page[kTableWrites];
 };
 static_assert(sizeof(PagedTableArgs) <= 4096, "kernel arguments exceed their limit");
+
+// Floats of a group's queries that the selection kernel stages where it takes them raw.
+constexpr uint32_t kSelectFloats = 8192;
 
 inline bool paged_supported(uint32_t d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 

@@ -53,22 +53,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
     *(float4_t*)&s_x[r][e] = *(const float4_t*)(src + (uint64_t)r * heads * D + e);
   }
   __syncthreads();
-  const float* w = is_q ? a.q_norm_w : is_k ? a.k_norm_w : nullptr;
-  const bool v_norm = !is_q && !is_k && a.v_norm != 0;
+  const float* w = is_q ? a.rot.q_norm_w : is_k ? a.rot.k_norm_w : nullptr;
+  const bool v_norm = !is_q && !is_k && a.rot.v_norm != 0;
   if (w != nullptr || v_norm) {
 #pragma clang fp contract(off)
-    if (threadIdx.x < n) {
-      const float* x = s_x[threadIdx.x];
-      float ss = 0.0f;
-#pragma unroll 4
-      for (int e = 0; e < D; e += 4) {
-        const float4_t v = *(const float4_t*)(x + e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ss = ss + v[i] * v[i];
-      }
-      const double mean = (double)(ss / (float)D + a.norm_eps);
-      s_scale[threadIdx.x] = v_norm ? (float)(1.0 / sqrt(mean)) : 1.0f / (float)sqrt(mean);
-    }
+    if (threadIdx.x < n) s_scale[threadIdx.x] = head_scale<D>(s_x[threadIdx.x], a.rot.norm_eps, v_norm);
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n * D; i += 256) {
       const uint32_t r = i / D, e = i % D;
@@ -78,16 +67,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
     }
     __syncthreads();
   }
-  if ((is_q || is_k) && a.cos_t != nullptr) {
-    for (uint32_t i = threadIdx.x; i < n * a.pairs; i += 256) {
-      const uint32_t r = i / a.pairs, j = i % a.pairs;
-      const uint64_t at = (uint64_t)(p0 + r) * a.pairs + j;
-      const uint32_t e0 = a.neox ? j : 2 * j, e1 = a.neox ? j + a.pairs : 2 * j + 1;
-      float x0 = s_x[r][e0], x1 = s_x[r][e1];
-      rotate_pair(x0, x1, a.cos_t[at], a.sin_t[at]);
-      s_x[r][e0] = x0;
-      s_x[r][e1] = x1;
-    }
+  if ((is_q || is_k) && a.rot.cos_t != nullptr) {
+    for (uint32_t i = threadIdx.x; i < n * a.rot.pairs; i += 256)
+      rotate_in(s_x[i / a.rot.pairs], i % a.rot.pairs, a.rot, p0 + i / a.rot.pairs);
     __syncthreads();
   }
   if (is_q) {
@@ -138,27 +120,24 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
   }
 }
 
-// Workgroup = (page that a chunk wrote to, kv head, chunk): the smallest and the largest of the page's
-// key elements, over all of its filled slots (those before the chunk's end). Exact, whatever the
-// order: no sums. A NaN key element is left out of them.
-template <typename KV, int D>
-__global__ __launch_bounds__(256) void paged_bounds_kernel(const PagedAppendArgs a) {
-  const PagedChunk c = a.c[blockIdx.z];
-  if (c.rows == 0) return;
-  const uint32_t number = (c.start >> a.kv.page_log2) + blockIdx.x, end = c.start + c.rows;
-  if (number > (end - 1) >> a.kv.page_log2) return;
-  const uint32_t filled = min(end - (number << a.kv.page_log2), 1u << a.kv.page_log2);
-  const uint32_t page = a.kv.table[(uint64_t)c.seq * a.kv.table_stride + number];
-  const uint32_t head = blockIdx.y;
-  const KV* src = (const KV*)a.kv.k + paged_base(page, a.kv.hkv, head, a.kv.page_log2, D);
+// The smallest and the largest of a page's key elements of one kv head, over its first `filled` slots, by a
+// workgroup of kThreads. Exact, whatever the order: no sums. A NaN key element is left out of them.
+// fresh: the last of these slots' keys in LDS (null: stored like the others). s_red: 2 * kThreads * 16
+// bytes / sizeof(KV) floats.
+template <typename KV, int D, uint32_t kThreads>
+__device__ __forceinline__ void page_bounds(const PagedView& kv, uint32_t page, uint32_t head, uint32_t filled,
+                                            const float* fresh, float* s_red) {
+  const KV* src = (const KV*)kv.k + paged_base(page, kv.hkv, head, kv.page_log2, D);
   constexpr bool kF16 = std::is_same<KV, _Float16>::value;
-  constexpr uint32_t kW = kF16 ? 8 : 4, kPieces = D / kW, kLanes = 256 / kPieces;
+  constexpr uint32_t kW = kF16 ? 8 : 4, kPieces = D / kW, kLanes = kThreads / kPieces;
   typedef KV kv16_t __attribute__((ext_vector_type(kW)));
   const uint32_t piece = threadIdx.x % kPieces, lane = threadIdx.x / kPieces;
   float lo[kW], hi[kW];
 #pragma unroll
   for (uint32_t t = 0; t < kW; ++t) lo[t] = INFINITY, hi[t] = -INFINITY;
-  for (uint32_t s = lane; s < filled; s += kLanes) {
+  const uint32_t stored = filled - (fresh ? 1u : 0u);
+#pragma unroll 4
+  for (uint32_t s = lane; s < stored; s += kLanes) {
     const kv16_t x = *(const kv16_t*)(src + paged_k_index(s, piece * kW, D, kF16));
 #pragma unroll
     for (uint32_t t = 0; t < kW; ++t) {
@@ -166,20 +145,37 @@ __global__ __launch_bounds__(256) void paged_bounds_kernel(const PagedAppendArgs
       hi[t] = fmaxf(hi[t], (float)x[t]);
     }
   }
-  __shared__ float s_lo[kLanes][D], s_hi[kLanes][D];
+  float* s_lo = s_red;
+  float* s_hi = s_red + kLanes * D;
 #pragma unroll
   for (uint32_t t = 0; t < kW; ++t) {
-    s_lo[lane][piece * kW + t] = lo[t];
-    s_hi[lane][piece * kW + t] = hi[t];
+    s_lo[lane * D + piece * kW + t] = lo[t];
+    s_hi[lane * D + piece * kW + t] = hi[t];
   }
   __syncthreads();
-  KV* dst = (KV*)a.kv.bounds + ((uint64_t)page * a.kv.hkv + head) * 2 * D;
-  for (uint32_t i = threadIdx.x; i < 2 * D; i += 256) {
+  KV* dst = (KV*)kv.bounds + ((uint64_t)page * kv.hkv + head) * 2 * D;
+  for (uint32_t i = threadIdx.x; i < 2 * D; i += kThreads) {
     const uint32_t e = i % D;
-    float x = i < D ? s_lo[0][e] : s_hi[0][e];
-    for (uint32_t l = 1; l < kLanes; ++l) x = i < D ? fminf(x, s_lo[l][e]) : fmaxf(x, s_hi[l][e]);
+    float x = i < D ? s_lo[e] : s_hi[e];
+    for (uint32_t l = 1; l < kLanes; ++l) x = i < D ? fminf(x, s_lo[l * D + e]) : fmaxf(x, s_hi[l * D + e]);
+    if (fresh) {
+      const float y = (float)(KV)fresh[e];
+      x = i < D ? fminf(x, y) : fmaxf(x, y);
+    }
     dst[i] = (KV)x;
   }
+}
+
+// Workgroup = (page that a chunk wrote to, kv head, chunk).
+template <typename KV, int D>
+__global__ __launch_bounds__(256) void paged_bounds_kernel(const PagedAppendArgs a) {
+  const PagedChunk c = a.c[blockIdx.z];
+  if (c.rows == 0) return;
+  const uint32_t number = (c.start >> a.kv.page_log2) + blockIdx.x, end = c.start + c.rows;
+  if (number > (end - 1) >> a.kv.page_log2) return;
+  __shared__ float s_red[2 * 256 * 16 / sizeof(KV)];
+  page_bounds<KV, D, 256>(a.kv, a.kv.table[(uint64_t)c.seq * a.kv.table_stride + number], blockIdx.y,
+                          min(end - (number << a.kv.page_log2), 1u << a.kv.page_log2), nullptr, s_red);
 }
 
 __global__ __launch_bounds__(512) void paged_table_kernel(const PagedTableArgs a) {
@@ -212,25 +208,25 @@ __device__ __forceinline__ double row_sum(double x) {
   return x;
 }
 
-constexpr uint32_t kPickRounds = 16, kPickPages = 256 * kPickRounds;  // keys a workgroup holds in registers
-
 // The pages of one (row, kv head), ascending: the first `first`, the last `last` and the `top` others of
 // the largest keys, of equal ones the lowest. The key of the last page taken is narrowed by eight
 // bits a pass, from the highest bit in which any two keys differ, until every key that shares the bits
 // found so far is taken (two or three passes: the keys are spread). n > first + last + top.
+template <uint32_t kPickRounds>
 __device__ __forceinline__ void pick_pages(const uint64_t* keys, uint32_t n, uint32_t top, uint32_t first, uint32_t last,
                                            uint32_t* out) {
   __shared__ uint32_t s_hist[256], s_found[3], s_any[4][2], s_sum[4];
-  __shared__ uint32_t s_count[4 * kPickRounds];
+  __shared__ uint32_t s_count[64];
+  constexpr uint32_t kPickPages = 256 * kPickRounds;  // keys the workgroup holds in registers
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint64_t k[kPickRounds];
   auto candidate = [&](uint32_t p) JMA_INL { return p >= first && p + last < n; };
   auto load = [&](uint32_t base) JMA_INL {
 #pragma unroll
     for (uint32_t i = 0; i < kPickRounds; ++i) {
-      const uint32_t p = base + 256 * i + tid;
-      k[i] = 0;
-      if (base + 256 * i < n && candidate(p)) k[i] = __hip_atomic_load(&keys[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      // Unconditional, so that all are in flight together: those of no candidate are not looked at.
+      const uint32_t p = min(base + 256 * i + tid, n - last - 1);
+      k[i] = __hip_atomic_load(&keys[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   };
   auto each = [&](auto&& f) JMA_INL {  // f(round's first page) over the keys, re-read where they are too many
@@ -350,7 +346,7 @@ __device__ __forceinline__ void pick_pages(const uint64_t* keys, uint32_t n, uin
       }
       __syncthreads();
       if (wave == 0) {
-        const uint32_t mine = s_count[lane];
+        const uint32_t mine = lane < 4 * kPickRounds ? s_count[lane] : 0;
         uint32_t sum = mine;
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) {
@@ -411,6 +407,8 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   }
   const uint64_t slot = ((uint64_t)blockIdx.z * a.max_rows + r) * hkv + kvh;
   uint64_t* keys = a.keys + slot * a.key_stride;
+  extern __shared__ __attribute__((aligned(16))) float s_queries[];  // raw: [group][D + 4]
+  __shared__ float s_scale[kSelectFloats / 32];
 
   constexpr int kE = D / 16, kP = kSelectPages / 16;
   typedef KV kve_t __attribute__((ext_vector_type(kE)));
@@ -426,7 +424,12 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
     lo[i] = *(const kve_t*)b;
     hi[i] = *(const kve_t*)(b + D);
   }
-  const float* q = a.q + ((uint64_t)row * a.num_heads + kvh * a.group) * D + lane16 * kE;
+  const float* q = a.q + ((uint64_t)row * a.num_heads + kvh * a.group) * D;
+  if (a.raw) {
+    for (uint32_t i = threadIdx.x; i < a.group * (D / 4); i += 256)
+      *(float4_t*)&s_queries[i / (D / 4) * (D + 4) + 4 * (i % (D / 4))] = *(const float4_t*)(q + 4 * i);
+    prepare_token<D, D + 4>(s_queries, s_scale, a.group, 0, false, a.rot, pos, 256);
+  }
   double best[kP];
   bool odd[kP];
 #pragma unroll
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   for (uint32_t h = 0; h < a.group; ++h) {
     float x[kE];
 #pragma unroll
-    for (int e = 0; e < kE; ++e) x[e] = q[(uint64_t)h * D + e];
+    for (int e = 0; e < kE; ++e) x[e] = a.raw ? s_queries[h * (D + 4) + lane16 * kE + e] : q[(uint64_t)h * D + lane16 * kE + e];
 #pragma unroll
     for (int i = 0; i < kP; ++i) {
       double s = 0.0;
@@ -462,7 +465,8 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
     if (s_last + 1 != wgs) return;
     if (threadIdx.x == 0) __hip_atomic_store(&a.tickets[slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  pick_pages(keys, n, a.top, a.first, a.last, out);
+  if (n <= 1024) pick_pages<4>(keys, n, a.top, a.first, a.last, out);
+  else pick_pages<16>(keys, n, a.top, a.first, a.last, out);
 }
 
 // ================================================================ attention
@@ -474,26 +478,75 @@ struct Step;
 template <int D>
 struct Step<_Float16, D> {
   half8_t k[2][D / 32], v[D / 16];
-  __device__ __forceinline__ void load(const _Float16* kt, const _Float16* vt, uint32_t, int c16, int g) {
+  __device__ __forceinline__ void load_k(const _Float16* kt, uint32_t, int c16, int g) {
     const uint32_t slot = 8 * (c16 >> 2) + (c16 & 3);
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) k[b][c] = *(const half8_t*)(kt + c * 1024 + (slot + 4 * b) * 32 + 8 * g);
+  }
+  __device__ __forceinline__ void load_v(const _Float16* vt, uint32_t, int c16, int g) {
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) v[n] = *(const half8_t*)(vt + (16 * n + c16) * 32 + 8 * g);
+  }
+  // Slot r of the step replaced by the key (value) in LDS.
+  __device__ __forceinline__ void patch_k(const float* x, uint32_t r, int c16, int g) {
+    const uint32_t slot = 8 * (c16 >> 2) + (c16 & 3);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[b][c][e] = slot + 4 * b == r ? (_Float16)x[32 * c + 8 * g + e] : k[b][c][e];
+  }
+  __device__ __forceinline__ void patch_v(const float* x, uint32_t r, int c16, int g) {
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      const _Float16 y = (_Float16)x[16 * n + c16];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[n][e] = r == (uint32_t)(8 * g + e) ? y : v[n][e];
+    }
   }
 };
 template <int D>
 struct Step<float, D> {
   float4_t k[D / 16], v[D / 16];
-  __device__ __forceinline__ void load(const float* kt, const float* vt, uint32_t half, int c16, int g) {
+  __device__ __forceinline__ void load_k(const float* kt, uint32_t half, int c16, int g) {
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) k[c] = *(const float4_t*)(kt + c * 512 + (16 * half + c16) * 16 + 4 * g);
+  }
+  __device__ __forceinline__ void load_v(const float* vt, uint32_t half, int c16, int g) {
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) v[n] = *(const float4_t*)(vt + (16 * n + c16) * 32 + 16 * half + 4 * g);
   }
+  __device__ __forceinline__ void patch_k(const float* x, uint32_t r, int c16, int g) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k[c][e] = (uint32_t)c16 == r ? x[16 * c + 4 * g + e] : k[c][e];
+  }
+  __device__ __forceinline__ void patch_v(const float* x, uint32_t r, int c16, int g) {
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[n][e] = r == (uint32_t)(4 * g + e) ? x[16 * n + c16] : v[n][e];
+  }
 };
+
+// The new token of a chunk of one row, stored by a workgroup of its own: K, V, and the bounds of their page.
+template <typename KV, int D, uint32_t kThreads>
+__device__ __forceinline__ void store_token(const PagedView& kv, const PagedChunk& ch, uint32_t kvh, const float* key,
+                                            const float* value, float* s_red) {
+  constexpr bool kF16 = std::is_same<KV, _Float16>::value;
+  const uint32_t page = kv.table[(uint64_t)ch.seq * kv.table_stride + (ch.start >> kv.page_log2)];
+  const uint32_t slot = ch.start & ((1u << kv.page_log2) - 1);
+  const uint64_t base = paged_base(page, kv.hkv, kvh, kv.page_log2, D);
+  for (uint32_t e = threadIdx.x; e < D; e += kThreads) {
+    ((KV*)kv.k)[base + paged_k_index(slot, e, D, kF16)] = (KV)key[e];
+    ((KV*)kv.v)[base + paged_v_index(slot, e, D)] = (KV)value[e];
+  }
+  if (kv.bounds != nullptr) page_bounds<KV, D, kThreads>(kv, page, kvh, slot + 1, key, s_red);
+}
 
 // Workgroup = (split, kv head x head group x block of query rows, chunk): 16 matrix-core columns =
 // (query row, query head) pairs that share every K/V load; its waves stride over the split's steps
@@ -509,17 +562,31 @@ struct Step<float, D> {
 // largest element in [2^13, 2^14), which costs nothing (the score's factor undoes it) and keeps both
 // halves far from f16's ends; p is formed as 2^(s - m + 6) for the same reason.
 //
-// Positions a column does not see are masked after the product, and values that are no finite number
-// in a step that is masked in part reach only the columns that see them (0 x inf is no 0), as NaN.
-template <typename KV, int D, bool kSelected>
+// kFused: the chunks are one token each, whose q, k and v come raw: every workgroup normalises and rotates
+// its queries, the one of the last split also the token's key, which it puts in place of the stored slot,
+// and one more workgroup per kv head (split = their count) stores the token, so that nobody waits for it.
+//
+// Positions a column does not see are masked after the product. A value that is no finite number, in a
+// step that a column sees in part, reaches all of the wave's columns (0 x inf is no 0); a wave with such an
+// output does its steps again, with those values taken out of the product and what they make of the
+// columns that see them (NaN) put in.
+template <typename KV, int D, bool kSelected, bool kFused>
 __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const PagedAttendArgs a) {
   constexpr bool kF16 = std::is_same<KV, _Float16>::value;
   constexpr int kW = paged_waves(D), kNs = kF16 ? 8 : 4, kNv = D / 16;
-  constexpr uint32_t kStep = kF16 ? 32 : 16;
-  constexpr int kQStride = D + 4;
-  __shared__ __attribute__((aligned(16))) float s_q[16][kQStride];
-  __shared__ __attribute__((aligned(16))) float s_acc[kW][16][D];
+  constexpr uint32_t kStep = kF16 ? 32 : 16, kThreads = 64 * kW;
+  constexpr int kQStride = D + 4, kHStride = D + 8;
+  // At heads of 256 a step's K and V take half the registers: only the next step's K is loaded ahead, and
+  // the queries' halves stay in LDS.
+  constexpr bool kWide = D >= 256;
+  __shared__ __attribute__((aligned(16))) float s_q[(kFused ? 18 : 16) * kQStride];
+  __shared__ __attribute__((aligned(16))) _Float16 s_qh[kWide && kF16 ? 2 * 16 * kHStride : 8];
+  // The waves' states; a storing workgroup's bounds (page_bounds) before.
+  constexpr int kAccFloats = kW * 16 * D, kRedFloats = kFused ? 2 * kThreads * 16 / sizeof(KV) : 0;
+  __shared__ __attribute__((aligned(16))) float s_acc_mem[kAccFloats > kRedFloats ? kAccFloats : kRedFloats];
+  float (*s_acc)[16][D] = (float (*)[16][D])s_acc_mem;
   __shared__ float s_ml[kW][16][2];
+  __shared__ float s_scale[18];
   __shared__ uint32_t s_ticket;
 
   const PagedChunk ch = a.c[blockIdx.z];
@@ -534,8 +601,12 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
   const uint32_t page_log2 = a.kv.page_log2;
   const uint32_t steps_log2 = page_log2 - (kF16 ? 5 : 4);  // steps of a page
   paged_range(pos0, pos1, a.window, kSelected ? a.budget : 0u, page_log2, kStep, t0, t1);
+  // A fused launch's lists end with the token's own page: its steps behind the token are left out, and the
+  // token is in the last split.
+  if (kSelected && kFused) t1 -= (1u << steps_log2) - 1 - (pos0 & ((1u << page_log2) - 1)) / kStep;
   const uint32_t ns = (t1 - t0 + a.tiles_per_split - 1) / a.tiles_per_split, split = blockIdx.x;
-  if (split >= ns) return;
+  if (split >= ns + (kFused && hg == 0 ? 1u : 0u)) return;
+  const bool stores = kFused && split == ns;  // the workgroup that appends the token
   t0 += split * a.tiles_per_split;
   t1 = min(t1, t0 + a.tiles_per_split);
 
@@ -546,71 +617,94 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
   const uint32_t cpos = pos0 + min(col_row, rows - 1), cfirst = first_visible(cpos, a.window);
   const uint64_t qrow = (uint64_t)ch.row0 + row0;
 
-  // q of the block's columns, in LDS.
-  const float* q = a.q + (qrow * a.num_heads + kvh * a.group + 16 * hg) * D;
-  for (uint32_t i = threadIdx.x; i < 16 * (D / 4); i += 64 * kW) {
-    const uint32_t c = i / (D / 4), e = 4 * (i % (D / 4)), r = c / heads, h = c % heads;
-    float4_t x = {0.f, 0.f, 0.f, 0.f};
-    if (r < rows) x = *(const float4_t*)(q + ((uint64_t)r * a.num_heads + h) * D + e);
-    *(float4_t*)&s_q[c][e] = x;
-  }
-
   // The page of each of this wave's next 64 steps is held by the lane of that number: its logical
   // number and where it is.
   const uint32_t* table = a.kv.table + (uint64_t)ch.seq * a.kv.table_stride;
   const uint32_t* list = kSelected ? a.pages + ((qrow * hkv) + kvh) * a.budget : nullptr;
+  // A list made by the caller may hold anything: numbers past the row's position, or not ascending, are
+  // reported and left out.
+  auto listed = [&](uint32_t i) JMA_INL -> uint32_t {
+    const uint32_t n = list[i], before = i == 0 ? 0u : list[i - 1];
+    if (n == kNoPage) return n;
+    if (n <= cpos >> page_log2 && (i == 0 || before < n)) return n;
+    report(a.err, kErrBadPage);
+    return kNoPage;
+  };
   uint32_t my_page = 0, my_number = 0;
   auto fetch_pages = [&](uint32_t t) JMA_INL {
     const uint32_t mine = t + lane * kW;
     my_page = kNoPage;
     if (mine < t1) {
-      if (kSelected) {
-        const uint32_t i = mine >> steps_log2;
-        my_number = list[i];
-        // A list made by the caller may hold anything: numbers past the row's position, or not
-        // ascending, are reported and left out.
-        if (my_number != kNoPage) {
-          const bool ok = my_number <= cpos >> page_log2 && (i == 0 || list[i - 1] < my_number);
-          if (!ok) report(a.err, kErrBadPage);
-          if (ok) my_page = table[my_number];
-        }
-      } else {
-        my_number = mine >> steps_log2;
-        my_page = table[my_number];
-      }
+      my_number = kSelected ? listed(mine >> steps_log2) : mine >> steps_log2;
+      if (!kSelected || my_number != kNoPage) my_page = table[my_number];
     }
   };
   const KV* kbase = (const KV*)a.kv.k;
   const KV* vbase = (const KV*)a.kv.v;
-  // Loads step t (the i-th since fetch_pages) and returns its first position, or kNoPage.
-  auto load = [&](Step<KV, D>& x, uint32_t t, uint32_t i) JMA_INL -> uint32_t {
-    const uint32_t page = __builtin_amdgcn_readlane(my_page, i);
-    const uint32_t number = __builtin_amdgcn_readlane(my_number, i);
-    if (page >= a.kv.pages) return kNoPage;
+  // Where step t, on `page`, is stored: its K (the V storage has the same shape).
+  auto place = [&](uint32_t t, uint32_t page) JMA_INL {
     const uint32_t in = t & ((1u << steps_log2) - 1), tile = kF16 ? in : in >> 1;
-    const uint64_t at = paged_base(page, hkv, kvh, page_log2, D) + tile * kTileSlots * D;
-    x.load(kbase + at, vbase + at, in & 1, c16, g);
-    return (number << page_log2) + in * kStep;
+    return paged_base(page, hkv, kvh, page_log2, D) + tile * kTileSlots * D;
+  };
+  struct Place {
+    uint64_t at;
+    uint32_t p0;  // the step's first position, kNoPage: the step has no page
+  };
+  // Step t, the i-th since fetch_pages.
+  auto placed = [&](uint32_t t, uint32_t i) JMA_INL {
+    const uint32_t page = __builtin_amdgcn_readlane(my_page, i), number = __builtin_amdgcn_readlane(my_number, i);
+    Place x;
+    x.p0 = page < a.kv.pages ? (number << page_log2) + (t & ((1u << steps_log2) - 1)) * kStep : kNoPage;
+    x.at = place(t, page < a.kv.pages ? page : 0u);
+    return x;
   };
 
   uint32_t t = t0 + wave;
-  Step<KV, D> cur, nxt;
-  uint32_t p_cur = kNoPage, p_nxt = kNoPage, i = 0;
-  if (t < t1) {
-    fetch_pages(t);
-    p_cur = load(cur, t, 0);
+  if (!stores && t < t1) fetch_pages(t);
+
+  // q of the block's columns, in LDS; the token's key and value behind them where they are needed.
+  const bool with_kv = kFused && split + 1 >= ns;
+  const float* q = a.q + (qrow * a.num_heads + kvh * a.group + 16 * hg) * D;
+  for (uint32_t i = threadIdx.x; i < 16 * (D / 4); i += kThreads) {
+    const uint32_t c = i / (D / 4), e = 4 * (i % (D / 4)), r = c / heads, h = c % heads;
+    float4_t x = {0.f, 0.f, 0.f, 0.f};
+    if (r < rows) x = *(const float4_t*)(q + ((uint64_t)r * a.num_heads + h) * D + e);
+    *(float4_t*)&s_q[c * kQStride + e] = x;
   }
+  if (with_kv && threadIdx.x < 2 * (D / 4)) {
+    const uint32_t i = threadIdx.x / (D / 4), e = 4 * (threadIdx.x % (D / 4));
+    *(float4_t*)&s_q[(16 + i) * kQStride + e] = *(const float4_t*)((i == 0 ? a.k_new : a.v_new) + (qrow * hkv + kvh) * D + e);
+  }
+
+  Step<KV, D> xa, xb;
+  Place pa = {0, kNoPage}, pb = {0, kNoPage};
+  uint32_t i = 0;
+  if (!stores && t < t1) {
+    pa = placed(t, 0);
+    const uint32_t half = t & 1;
+    xa.load_k(kbase + pa.at, half, c16, g);
+    if (!kWide) xa.load_v(vbase + pa.at, half, c16, g);
+  }
+  if constexpr (kFused) prepare_token<D, kQStride>(s_q, s_scale, heads, 16, with_kv, a.rot, pos0, kThreads);
+  const float* new_k = s_q + 16 * kQStride;
+  const float* new_v = s_q + 17 * kQStride;
+  if (stores) {
+    __syncthreads();
+    store_token<KV, D, kThreads>(a.kv, ch, kvh, new_k, new_v, s_acc_mem);
+    return;
+  }
+  const uint32_t new_p0 = kFused ? pos0 / kStep * kStep : kNoPage - 1, new_r = pos0 % kStep;
   __syncthreads();
 
   // Q operand and the factor of each column's scores.
-  half8_t qhi[kF16 ? D / 32 : 1], qlo[kF16 ? D / 32 : 1];
+  half8_t qhi[kF16 && !kWide ? D / 32 : 1], qlo[kF16 && !kWide ? D / 32 : 1];
   float4_t qf[kF16 ? 1 : D / 16];
   float factor = a.scale;
   if constexpr (kF16) {
     float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
-      const float4_t x0 = *(const float4_t*)&s_q[c16][32 * c + 8 * g], x1 = *(const float4_t*)&s_q[c16][32 * c + 8 * g + 4];
+      const float4_t x0 = *(const float4_t*)&s_q[c16 * kQStride + 32 * c + 8 * g], x1 = *(const float4_t*)&s_q[c16 * kQStride + 32 * c + 8 * g + 4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(x0[e]), fabsf(x1[e])));
     }
@@ -621,17 +715,28 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
     factor = __builtin_amdgcn_ldexpf(a.scale, ex - 14);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
-      const float4_t x0 = *(const float4_t*)&s_q[c16][32 * c + 8 * g], x1 = *(const float4_t*)&s_q[c16][32 * c + 8 * g + 4];
+      if (kWide && c % kW != wave) continue;
+      const float4_t x0 = *(const float4_t*)&s_q[c16 * kQStride + 32 * c + 8 * g], x1 = *(const float4_t*)&s_q[c16 * kQStride + 32 * c + 8 * g + 4];
+      half8_t yh, yl;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = __builtin_amdgcn_ldexpf(e < 4 ? x0[e & 3] : x1[e & 3], 14 - ex);
-        qhi[c][e] = (_Float16)x;
-        qlo[c][e] = (_Float16)(x - (float)qhi[c][e]);
+        _Float16 hi, lo;
+        halves(__builtin_amdgcn_ldexpf(e < 4 ? x0[e & 3] : x1[e & 3], 14 - ex), hi, lo);
+        yh[e] = hi;
+        yl[e] = lo;
+      }
+      if constexpr (kWide) {
+        *(half8_t*)&s_qh[c16 * kHStride + 32 * c + 8 * g] = yh;
+        *(half8_t*)&s_qh[(16 + c16) * kHStride + 32 * c + 8 * g] = yl;
+      } else {
+        qhi[c] = yh;
+        qlo[c] = yl;
       }
     }
+    if constexpr (kWide) __syncthreads();
   } else {
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) qf[c] = *(const float4_t*)&s_q[c16][16 * c + 4 * g];
+    for (int c = 0; c < D / 16; ++c) qf[c] = *(const float4_t*)&s_q[c16 * kQStride + 16 * c + 4 * g];
   }
 
   float m = -INFINITY, l = 0.0f;  // of this lane's slots, maximum in log2 units shared by the column
@@ -639,29 +744,32 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
 #pragma unroll
   for (int n = 0; n < kNv; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-  auto step = [&](const Step<KV, D>& x, uint32_t p0) JMA_INL {
-    float4_t s[kF16 ? 2 : 1];
+  // Scores of the step at p0; the products are left to step().
+  auto scores = [&](const Step<KV, D>& x, float (&sc)[kNs]) JMA_INL {
+    float4_t s[kF16 ? 2 : 1] = {};
+    if constexpr (kF16) {
 #pragma unroll
-    for (int b = 0; b < (kF16 ? 2 : 1); ++b) {
-      s[b] = float4_t{0.f, 0.f, 0.f, 0.f};
-      if constexpr (kF16) {
+      for (int c = 0; c < D / 32; ++c) {
+        const half8_t hi = kWide ? *(const half8_t*)&s_qh[c16 * kHStride + 32 * c + 8 * g] : qhi[kWide ? 0 : c];
+        const half8_t lo = kWide ? *(const half8_t*)&s_qh[(16 + c16) * kHStride + 32 * c + 8 * g] : qlo[kWide ? 0 : c];
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[b][c], qlo[c], s[b], 0, 0, 0);
+        for (int b = 0; b < 2; ++b) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[b][c], lo, s[b], 0, 0, 0);
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[b][c], qhi[c], s[b], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[c][e], qf[c][e], s[b], 0, 0, 0);
+        for (int b = 0; b < 2; ++b) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[b][c], hi, s[b], 0, 0, 0);
       }
-    }
-    const bool whole = p0 + kStep - 1 <= pos0 && p0 >= first_visible(pos1, a.window);
-    float sc[kNs];
+    } else {
 #pragma unroll
-    for (int e = 0; e < kNs; ++e) {
-      sc[e] = s[e >> 2][e & 3];
-      if (!whole) {
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[c][e], qf[c][e], s[0], 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < kNs; ++e) sc[e] = s[e >> 2][e & 3];
+  };
+  auto step = [&](Step<KV, D>& x, uint32_t p0, float (&sc)[kNs], auto robust) JMA_INL {
+    if (p0 + kStep - 1 > pos0 || p0 < first_visible(pos1, a.window)) {
+#pragma unroll
+      for (int e = 0; e < kNs; ++e) {
         const uint32_t p = p0 + kNs * g + e;
         sc[e] = p >= cfirst && p <= cpos ? sc[e] : -INFINITY;
       }
@@ -680,7 +788,7 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
 #pragma unroll
       for (int n = 0; n < kNv; ++n) acc[n] *= alpha;
     }
-    const float shift = kF16 ? 6.0f - (m == -INFINITY ? 0.0f : m) : (m == -INFINITY ? 0.0f : -m);
+    const float shift = (kF16 ? 6.0f : 0.0f) - (m == -INFINITY ? 0.0f : m);
     float pr[kNs];
 #pragma unroll
     for (int e = 0; e < kNs; ++e) {
@@ -691,8 +799,10 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
     if constexpr (kF16) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        ph[e] = (_Float16)pr[e];
-        pl[e] = (_Float16)(pr[e] - (float)ph[e]);
+        _Float16 hi, lo;
+        halves(pr[e], hi, lo);
+        ph[e] = hi;
+        pl[e] = lo;
       }
     }
     auto product = [&](const auto& v, float4_t o) JMA_INL {
@@ -705,54 +815,107 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
       }
       return o;
     };
-    if (!whole) {
-      // Values here that are no finite number are left out of the product, and what they make of the
-      // columns that see them is added: a second product counts, for each output, the ones its column sees.
-      uint32_t odd = 0;
+    if constexpr (decltype(robust)::value) {
+      std::conditional_t<kF16, half8_t, float4_t> sees;
 #pragma unroll
-      for (int n = 0; n < kNv; ++n) odd |= not_finite(x.v[n]);
-      if (__ballot(odd != 0) != 0) {
-        std::conditional_t<kF16, half8_t, float4_t> sees;
-#pragma unroll
-        for (int e = 0; e < kNs; ++e) {
-          const uint32_t p = p0 + kNs * g + e;
-          sees[e] = p >= cfirst && p <= cpos ? 1.0f : 0.0f;
-        }
-#pragma unroll
-        for (int n = 0; n < kNv; ++n) {
-          auto v = x.v[n], is = x.v[n];
-          split_finite(v, is);
-          float4_t count = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (kF16) {
-            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees, count, 0, 0, 0);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) count = __builtin_amdgcn_mfma_f32_16x16x4f32(is[e], sees[e], count, 0, 0, 0);
-          }
-          acc[n] = product(v, acc[n]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][e] = count[e] > 0.0f ? NAN : acc[n][e];
-        }
-        return;
+      for (int e = 0; e < kNs; ++e) {
+        const uint32_t p = p0 + kNs * g + e;
+        sees[e] = p >= cfirst && p <= cpos ? 1.0f : 0.0f;
       }
-    }
 #pragma unroll
-    for (int n = 0; n < kNv; ++n) acc[n] = product(x.v[n], acc[n]);
+      for (int n = 0; n < kNv; ++n) {
+        auto is = x.v[n];
+        split_finite(x.v[n], is);
+        float4_t found = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (kF16) {
+          found = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees, found, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) found = __builtin_amdgcn_mfma_f32_16x16x4f32(is[e], sees[e], found, 0, 0, 0);
+        }
+        acc[n] = product(x.v[n], acc[n]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] = found[e] > 0.0f ? NAN : acc[n][e];
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < kNv; ++n) acc[n] = product(x.v[n], acc[n]);
+    }
   };
-
-  while (t < t1) {
+  // Step x at p; the next one, y, is loaded meanwhile.
+  auto half_loop = [&](Step<KV, D>& x, const Place& px, Step<KV, D>& y, Place& py) JMA_INL {
     const uint32_t tn = t + kW;
-    if (tn < t1) {
+    if (!kWide && tn < t1) {
       if (++i == 64) {
         fetch_pages(tn);
         i = 0;
       }
-      p_nxt = load(nxt, tn, i);
+      py = placed(tn, i);
+      y.load_k(kbase + py.at, tn & 1, c16, g);
+      y.load_v(vbase + py.at, tn & 1, c16, g);
     }
-    if (p_cur != kNoPage) step(cur, p_cur);
-    cur = nxt;
-    p_cur = p_nxt;
+    float sc[kNs];
+    const uint32_t p0 = px.p0;
+    if (kWide) x.load_v(vbase + px.at, t & 1, c16, g);
+    if (kFused && p0 == new_p0) {
+      x.patch_k(new_k, new_r, c16, g);
+      x.patch_v(new_v, new_r, c16, g);
+    }
+    scores(x, sc);
+    if (kWide && tn < t1) {
+      if (++i == 64) {
+        fetch_pages(tn);
+        i = 0;
+      }
+      py = placed(tn, i);
+      x.load_k(kbase + py.at, tn & 1, c16, g);
+    }
+    if (p0 != kNoPage) step(x, p0, sc, std::false_type{});
     t = tn;
+  };
+  const uint32_t t_first = t;
+  if constexpr (kWide) {
+    while (t < t1) {
+      Place next = {0, kNoPage};
+      half_loop(xa, pa, xa, next);
+      pa = next;
+    }
+  } else {
+    while (t < t1) {
+      half_loop(xa, pa, xb, pb);
+      if (t >= t1) break;
+      half_loop(xb, pb, xa, pa);
+    }
+  }
+
+  float odd = 0.0f;
+#pragma unroll
+  for (int n = 0; n < kNv; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd = fmaf(acc[n][e], 0.0f, odd);
+  if (__ballot(odd != 0.0f) != 0) {
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int n = 0; n < kNv; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (t = t_first; t < t1; t += kW) {
+      const uint32_t number = __builtin_amdgcn_readfirstlane(kSelected ? listed(t >> steps_log2) : t >> steps_log2);
+      if (number == kNoPage) continue;
+      const uint32_t page = __builtin_amdgcn_readfirstlane(table[number]);
+      if (page >= a.kv.pages) continue;
+      const uint32_t p0 = (number << page_log2) + (t & ((1u << steps_log2) - 1)) * kStep;
+      const uint64_t at = place(t, page);
+      xa.load_k(kbase + at, t & 1, c16, g);
+      xa.load_v(vbase + at, t & 1, c16, g);
+      if (kFused && p0 == new_p0) {
+        xa.patch_k(new_k, new_r, c16, g);
+        xa.patch_v(new_v, new_r, c16, g);
+      }
+      float sc[kNs];
+      scores(xa, sc);
+      step(xa, p0, sc, std::true_type{});
+    }
   }
 
   // The waves' states meet in LDS.
@@ -776,7 +939,7 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
     if (e == 0 && !(sum > 0.0f && sum < INFINITY)) report(a.err, kErrNonFinite);
     *(float4_t*)(out + ((uint64_t)r * a.num_heads + h) * D + e) = o * (sum > 0.0f ? 1.0f / sum : sum);
   };
-  for (uint32_t k = threadIdx.x; k < cols * (D / 4); k += 64 * kW) {
+  for (uint32_t k = threadIdx.x; k < cols * (D / 4); k += kThreads) {
     const uint32_t c = k / (D / 4), e = 4 * (k % (D / 4));
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
@@ -808,30 +971,30 @@ __global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const
   if (s_ticket + 1 != ns) return;
   if (threadIdx.x == 0) __hip_atomic_store(&a.tickets[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // Two round trips: every split's (m, l), and its share of O, eight splits' words in flight.
-  float (*s_all)[16][2] = (float (*)[16][2])s_acc;  // [split][column]
-  for (uint32_t k = threadIdx.x; k < ns * 16; k += 64 * kW) {
+  float (*s_all)[16][2] = (float (*)[16][2])s_acc_mem;  // [split][column]
+  for (uint32_t k = threadIdx.x; k < ns * 16; k += kThreads) {
     const float4_t ml = load_part(rs, ((k / 16 * 16 + min(k % 16, cols - 1)) * (D + 4) + D) * 4);
     s_all[k / 16][k % 16][0] = ml[0];
     s_all[k / 16][k % 16][1] = ml[1];
   }
   __syncthreads();
-  for (uint32_t k = threadIdx.x; k < cols * (D / 4); k += 64 * kW) {
+  for (uint32_t k = threadIdx.x; k < cols * (D / 4); k += kThreads) {
     const uint32_t c = k / (D / 4), e = 4 * (k % (D / 4));
     float M = -INFINITY, L = 0.0f;
     float4_t o = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t s0 = 0; s0 < ns; s0 += 8) {
       float4_t x[8];
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) x[i] = load_part(rs, ((min(s0 + i, ns - 1) * 16 + c) * (D + 4) + e) * 4);
+      for (uint32_t i8 = 0; i8 < 8; ++i8) x[i8] = load_part(rs, ((min(s0 + i8, ns - 1) * 16 + c) * (D + 4) + e) * 4);
       if (s0 == 0)
         for (uint32_t s = 0; s < ns; ++s) M = fmaxf(M, s_all[s][c][0]);
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) {
-        if (s0 + i >= ns) break;
-        const float ms = s_all[s0 + i][c][0], f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
-        L = fmaf(s_all[s0 + i][c][1], f, L);
+      for (uint32_t i8 = 0; i8 < 8; ++i8) {
+        if (s0 + i8 >= ns) break;
+        const float ms = s_all[s0 + i8][c][0], f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
+        L = fmaf(s_all[s0 + i8][c][1], f, L);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(x[i][j], f, o[j]);
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(x[i8][j], f, o[j]);
       }
     }
     finish(c, e, o, L);
@@ -873,7 +1036,8 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, u
     using KV = decltype(kv);
     constexpr int D = decltype(dim)::value;
     const uint32_t wgs = (max_pages + kSelectPages - 1) / kSelectPages;
-    paged_select_kernel<KV, D><<<dim3(wgs, a.max_rows * a.kv.hkv, a.chunks), 256, 0, stream>>>(a);
+    const uint32_t lds = a.raw ? a.group * (D + 4) * 4 : 0;
+    paged_select_kernel<KV, D><<<dim3(wgs, a.max_rows * a.kv.hkv, a.chunks), 256, lds, stream>>>(a);
     return hipGetLastError();
   });
 }
@@ -882,9 +1046,13 @@ hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, h
   return by_shape(f16, d, [&](auto kv, auto dim) {
     using KV = decltype(kv);
     constexpr int D = decltype(dim)::value;
-    const dim3 grid(a.max_splits, a.max_blocks * a.kv.hkv * a.head_groups, a.chunks);
-    if (a.pages != nullptr) paged_attend_kernel<KV, D, true><<<grid, 64 * paged_waves(D), 0, stream>>>(a);
-    else paged_attend_kernel<KV, D, false><<<grid, 64 * paged_waves(D), 0, stream>>>(a);
+    const bool fused = a.k_new != nullptr;
+    const dim3 grid(a.max_splits + (fused ? 1 : 0), a.max_blocks * a.kv.hkv * a.head_groups, a.chunks);
+    constexpr uint32_t kThreads = 64 * paged_waves(D);
+    if (fused && a.pages != nullptr) paged_attend_kernel<KV, D, true, true><<<grid, kThreads, 0, stream>>>(a);
+    else if (fused) paged_attend_kernel<KV, D, false, true><<<grid, kThreads, 0, stream>>>(a);
+    else if (a.pages != nullptr) paged_attend_kernel<KV, D, true, false><<<grid, kThreads, 0, stream>>>(a);
+    else paged_attend_kernel<KV, D, false, false><<<grid, kThreads, 0, stream>>>(a);
     return hipGetLastError();
   });
 }

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -31,6 +32,65 @@ __device__ __forceinline__ void rotate_pair(float& x0, float& x1, float c, float
   const float y0 = x0 * c - x1 * s, y1 = x0 * s + x1 * c;
   x0 = y0;
   x1 = y1;
+}
+
+// 1 / rms of a head in LDS, its sum of squares in order (TensorOps.rmsNorm); value: the norm without a
+// weight (Gemma4Math.normalizeWithoutWeight).
+template <int D>
+__device__ __forceinline__ float head_scale(const float* x, float eps, bool value) {
+#pragma clang fp contract(off)
+  float ss = 0.0f;
+#pragma unroll 4
+  for (int e = 0; e < D; e += 4) {
+    const float4_t v = *(const float4_t*)(x + e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss = ss + v[i] * v[i];
+  }
+  const double mean = (double)(ss / (float)D + eps);
+  return value ? (float)(1.0 / sqrt(mean)) : 1.0f / (float)sqrt(mean);
+}
+
+// Pair j of a head in LDS, rotated with the factors of its position (RoPE row `at`).
+__device__ __forceinline__ void rotate_in(float* x, uint32_t j, const PagedRotation& r, uint64_t at) {
+  const uint32_t e0 = r.neox ? j : 2 * j, e1 = r.neox ? j + r.pairs : 2 * j + 1;
+  float x0 = x[e0], x1 = x[e1];
+  rotate_pair(x0, x1, r.cos_t[at * r.pairs + j], r.sin_t[at * r.pairs + j]);
+  x[e0] = x0;
+  x[e1] = x1;
+}
+
+// The query heads (rows 0 .. heads - 1 of s) of one token, and where `with_kv` its key and value of one kv
+// head (rows kv0, kv0 + 1), normalised and rotated in LDS by the whole workgroup. Ends with a barrier.
+template <int D, int kStride>
+__device__ __forceinline__ void prepare_token(float* s, float* s_scale, uint32_t heads, uint32_t kv0, bool with_kv,
+                                              const PagedRotation& r, uint32_t pos, uint32_t threads) {
+  __syncthreads();
+  const uint32_t tid = threadIdx.x, rows = heads + (with_kv ? 2u : 0u);
+  auto row_of = [&](uint32_t i) JMA_INL { return i < heads ? i : kv0 + i - heads; };
+  if (r.q_norm_w != nullptr || r.k_norm_w != nullptr || r.v_norm != 0) {
+#pragma clang fp contract(off)
+    if (tid < rows) {
+      const bool value = tid == heads + 1;
+      if (tid < heads ? r.q_norm_w != nullptr : value ? r.v_norm != 0 : r.k_norm_w != nullptr)
+        s_scale[tid] = head_scale<D>(s + row_of(tid) * kStride, r.norm_eps, value);
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < rows * D; i += threads) {
+      const uint32_t row = i / D, e = i % D;
+      const bool value = row == heads + 1;
+      const float* w = row < heads ? r.q_norm_w : r.k_norm_w;
+      if (value ? r.v_norm == 0 : w == nullptr) continue;
+      float* x = s + row_of(row) * kStride + e;
+      const float y = *x * s_scale[row];
+      *x = value ? y : y * w[e];
+    }
+    __syncthreads();
+  }
+  if (r.cos_t != nullptr) {
+    for (uint32_t i = tid; i < (heads + (with_kv ? 1u : 0u)) * r.pairs; i += threads)
+      rotate_in(s + row_of(i / r.pairs) * kStride, i % r.pairs, r, pos);
+    __syncthreads();
+  }
 }
 
 __device__ __forceinline__ void swap16(float x, float& a, float& b) {

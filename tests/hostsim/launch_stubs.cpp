@@ -290,6 +290,12 @@ void check_pages(const PagedView& kv, uint32_t seq, uint32_t from, uint32_t to, 
   }
 }
 
+void check_rotation(const PagedRotation& r, uint64_t position) {
+  if (r.cos_t == nullptr) return;
+  check(r.cos_t, (position + 1) * r.pairs * 4, "rope cos");
+  check(r.sin_t, (position + 1) * r.pairs * 4, "rope sin");
+}
+
 void check_grid(uint64_t x, uint64_t y, uint64_t z) {
   if (x == 0 || y == 0 || z == 0 || x > 0x7FFFFFFFu || y > 65535 || z > 65535) hipsim_fail("grid out of range");
 }
@@ -323,10 +329,7 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, h
       }
       check(a.k + c.row0 * kd, c.rows * kd * 4, "k");
       check(a.v + c.row0 * kd, c.rows * kd * 4, "v");
-      if (a.cos_t) {
-        check(a.cos_t, ((uint64_t)last + 1) * a.pairs * 4, "rope cos");
-        check(a.sin_t, ((uint64_t)last + 1) * a.pairs * 4, "rope sin");
-      }
+      check_rotation(a.rot, last);
       check_pages(a.kv, c.seq, c.start >> a.kv.page_log2, last >> a.kv.page_log2, d, es);
     }
   });
@@ -343,6 +346,8 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, u
       const PagedChunk& c = a.c[i];
       const uint32_t last = (c.start + c.rows - 1) >> a.kv.page_log2;
       if (c.rows > a.max_rows || last >= a.key_stride || last >= max_pages) hipsim_fail("chunk past the launch's sizes");
+      if (a.raw) check_rotation(a.rot, c.start + c.rows - 1);
+      if (a.raw && a.group * (d + 4) > kSelectFloats) hipsim_fail("raw queries past the kernel's room");
       check(a.q + (uint64_t)c.row0 * a.num_heads * d, (uint64_t)c.rows * a.num_heads * d * 4, "q");
       check(a.pages + (uint64_t)c.row0 * a.kv.hkv * a.budget, (uint64_t)c.rows * a.kv.hkv * a.budget * 4, "selected pages");
       check_pages(a.kv, c.seq, 0, last, d, f16 ? 2 : 4);
@@ -364,6 +369,12 @@ hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, h
       const uint64_t qd = (uint64_t)a.num_heads * d;
       check(a.q + c.row0 * qd, c.rows * qd * 4, "q");
       check(a.out + c.row0 * qd, c.rows * qd * 4, "out");
+      if (a.k_new) {
+        if (c.rows != 1) hipsim_fail("a fused launch with a chunk of more than one row");
+        check(a.k_new + (uint64_t)c.row0 * a.kv.hkv * d, (uint64_t)a.kv.hkv * d * 4, "new k");
+        check(a.v_new + (uint64_t)c.row0 * a.kv.hkv * d, (uint64_t)a.kv.hkv * d * 4, "new v");
+        check_rotation(a.rot, c.start);
+      }
       if (a.pages) check(a.pages + (uint64_t)c.row0 * a.kv.hkv * a.budget, (uint64_t)c.rows * a.kv.hkv * a.budget * 4, "selected pages");
       const uint32_t blocks = (c.rows + a.rows_per_block - 1) / a.rows_per_block;
       if (blocks > a.max_blocks) hipsim_fail("chunk of more blocks than the grid");
