@@ -61,11 +61,12 @@ JMA_HD uint32_t adapter_few_rows(uint32_t cols) {
   return fit < 4u ? fit : 4u;
 }
 // Rows and outputs of a workgroup's tile in the two-launch form.
-constexpr uint32_t kDownRows = 32, kUpRows = 64, kUpOuts = 128;
-// Pieces of the columns, so that few row blocks still fill the compute units: at least 256 columns each.
+constexpr uint32_t kDownRows = 16, kUpRows = 32, kUpOuts = 128;
+// Pieces of the columns: as many as keep the first product's workgroups (one a compute unit) in one round,
+// at least 512 columns each.
 inline uint32_t adapter_splits(uint32_t cols, uint64_t row_blocks, uint32_t cus) {
-  const uint64_t want = (2ull * cus + row_blocks - 1) / std::max<uint64_t>(row_blocks, 1);
-  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({want, 16ull, std::max(1u, cols / 256)}));
+  const uint64_t want = cus / std::max<uint64_t>(row_blocks, 1);
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({want, 16ull, std::max(1u, cols / 512)}));
 }
 
 }  // namespace jma

@@ -151,13 +151,14 @@ __global__ __launch_bounds__(512) void adapter_few_kernel(const AdapterArgs a) {
     if ((uint32_t)i < rows) a.out[at + (uint64_t)i * a.outs] = (a.base ? a.base[at + (uint64_t)i * a.outs] : 0.0f) + sum[i];
 }
 
-// Workgroup = (piece of the columns, 32 rows of a run, run): A x over that piece. Its four waves take a
-// quarter of the piece each and meet in LDS. One 16x16x4 product takes 16 ranks x 16 rows over four
-// columns; lane (g, c) holds eight neighbouring columns 8g .. 8g+7 of its row of either operand per step of
-// 32, so both are read in wide loads. Bound by reading x: ranks are taken 64 at a time, which is all of
-// them for most adapters.
+// Workgroup = (piece of the columns, 16 rows of a run, run): A x over that piece. Its eight waves take an
+// eighth of the piece each and meet in LDS, so that few pieces, which the second launch has to sum, fill
+// the device. One 16x16x4 product takes 16 ranks x 16 rows over four columns; lane (g, c) holds eight
+// neighbouring columns 8g .. 8g+7 of its row of either operand per step of 32, so both are read in wide
+// loads, two steps ahead. Bound by reading x: ranks are taken 64 at a time, which is all of them for most
+// adapters.
 template <uint32_t kType>
-__global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterArgs a) {
+__global__ __launch_bounds__(512) void adapter_down_kernel(const AdapterArgs a) {
   const AdapterRun run = a.run[blockIdx.z];
   const uint32_t r0 = blockIdx.y * kDownRows;
   if (run.rank16 == 0 || r0 >= run.rows) return;
@@ -165,65 +166,84 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterArgs a) 
   const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t c0 = blockIdx.x * a.cols_per_split, c1 = min(c0 + a.cols_per_split, a.cols);
-  const uint32_t quarter = ((c1 - c0 + 3) / 4 + 31) / 32 * 32;
-  const uint32_t w0 = min(c0 + wave * quarter, c1), w1 = min(w0 + quarter, c1);
-  __shared__ __attribute__((aligned(16))) float s_part[4][2][4][64][4];  // [wave][row tile][rank tile][lane]
+  const uint32_t eighth = ((c1 - c0 + 7) / 8 + 31) / 32 * 32;
+  const uint32_t w0 = min(c0 + wave * eighth, c1), w1 = min(w0 + eighth, c1);
+  __shared__ __attribute__((aligned(16))) float s_part[8][4][64][4];  // [wave][rank tile][lane]
   // Rows behind the run's last repeat it; their columns of the product are not stored.
-  const float* x[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) x[t] = a.x + (uint64_t)(run.row0 + r0 + min(16u * t + c16, rows - 1)) * a.cols + 8 * g;
-  for (uint32_t rank0 = 0; rank0 < run.rank16; rank0 += 64) {
-    const uint32_t tiles = min(4u, (run.rank16 - rank0) / 16);
-    float4_t acc[2][4] = {};
-    auto step = [&](uint32_t c, auto whole) JMA_INL {
+  const float* x = a.x + (uint64_t)(run.row0 + r0 + min(c16, rows - 1)) * a.cols;
+  // `tiles` tiles of 16 ranks from rank0 on. (Known when compiled: a load under a branch would be waited for
+  // where the branch ends.)
+  auto take = [&](uint32_t rank0, auto count) JMA_INL {
+    constexpr int kTiles = decltype(count)::value;
+    struct Operands {  // two steps
       float4_t v[2][2];
+      Raw<kType, 8> w[2][kTiles];
+    };
+    const uint64_t wrow = run.a_at + (uint64_t)(rank0 + c16) * a.cols;
+    float4_t acc[kTiles] = {};
+    // Columns past the piece's end read its first ones and count as zero.
+    auto load = [&](Operands& y, uint32_t c) JMA_INL {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t at = c + 32 * i + 8 * g < w1 ? c + 32 * i + 8 * g : c0;
+        y.v[i][0] = *(const float4_t*)(x + at);
+        y.v[i][1] = *(const float4_t*)(x + at + 4);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          v[t][i] = float4_t{0.f, 0.f, 0.f, 0.f};
-          if (decltype(whole)::value || c + 8 * g < w1) v[t][i] = *(const float4_t*)(x[t] + c + 4 * i);
-        }
-      Raw<kType, 8> w[4];
-#pragma unroll
-      for (uint32_t n = 0; n < 4; ++n) {
-        w[n].w = {};
-        if (n < tiles && (decltype(whole)::value || c + 8 * g < w1))
-          w[n].load(a.a, run.a_at + (uint64_t)(rank0 + 16 * n + c16) * a.cols + c + 8 * g);
+        for (int n = 0; n < kTiles; ++n) y.w[i][n].load(a.a, wrow + (uint64_t)16 * n * a.cols + at);
       }
+    };
+    auto products = [&](Operands& y, uint32_t c) JMA_INL {
 #pragma unroll
-      for (uint32_t n = 0; n < 4; ++n) {
-        if (n >= tiles) break;
+      for (uint32_t i = 0; i < 2; ++i) {
+        const bool in = c + 32 * i + 8 * g < w1;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[n][e], v[t][e / 4][e % 4], acc[t][n], 0, 0, 0);
+          for (int n = 0; n < kTiles; ++n)
+            acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? y.w[i][n][e] : 0.0f, in ? y.v[i][e / 4][e % 4] : 0.0f, acc[n], 0, 0, 0);
       }
     };
-    uint32_t c = w0;
-    for (; c + 32 <= w1; c += 32) step(c, std::true_type{});
-    if (c < w1) step(c, std::false_type{});
+    Operands ya, yb;
+    if (w0 < w1) {
+      load(ya, w0);
+      for (uint32_t c = w0;; c += 128) {
+        load(yb, c + 64);
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead of the products
+        products(ya, c);
+        if (c + 64 >= w1) break;
+        load(ya, c + 128);
+        __builtin_amdgcn_sched_barrier(0);
+        products(yb, c + 64);
+        if (c + 128 >= w1) break;
+      }
+    }
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (uint32_t n = 0; n < 4; ++n) *(float4_t*)s_part[wave][t][n][lane] = acc[t][n];
+    for (int n = 0; n < kTiles; ++n) *(float4_t*)s_part[wave][n][lane] = acc[n];
     __syncthreads();
     // Lane (g, c) of a tile holds ranks 4g .. 4g+3 of row c.
-    for (uint32_t i = threadIdx.x; i < 2 * tiles * 64; i += 256) {
-      const uint32_t l = i % 64, n = i / 64 % tiles, t = i / 64 / tiles, row = 16 * t + (l & 15);
-      float4_t sum = *(const float4_t*)s_part[0][t][n][l];
+    if (threadIdx.x < kTiles * 64) {
+      const uint32_t l = threadIdx.x % 64, n = threadIdx.x / 64, row = l & 15;
+      float4_t sum = *(const float4_t*)s_part[0][n][l];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) sum += *(const float4_t*)s_part[w][t][n][l];
+      for (int w = 1; w < 8; ++w) sum += *(const float4_t*)s_part[w][n][l];
       if (row < rows)
         *(float4_t*)&a.down[((uint64_t)(run.row0 + r0 + row) * a.splits + blockIdx.x) * a.max_rank16 + rank0 + 16 * n + 4 * (l >> 4)] = sum;
     }
+  };
+  for (uint32_t rank0 = 0; rank0 < run.rank16; rank0 += 64) {
+    const uint32_t tiles = min(4u, (run.rank16 - rank0) / 16);
+    if (tiles == 4) take(rank0, std::integral_constant<int, 4>{});
+    else if (tiles == 3) take(rank0, std::integral_constant<int, 3>{});
+    else if (tiles == 2) take(rank0, std::integral_constant<int, 2>{});
+    else take(rank0, std::integral_constant<int, 1>{});
   }
 }
 
-// Workgroup = (128 outputs, 64 rows of a run, run): base + scale B (A x), the pieces of A x summed in order
+// Workgroup = (128 outputs, 32 rows of a run, run): base + scale B (A x), the pieces of A x summed in order
 // into LDS first. A wave takes 32 outputs; a 16x16x4 product leaves lane (g, c) four neighbouring outputs
-// of row c, one 16-byte access each of base and out. Bound by reading base and writing out.
+// of row c, which go through LDS, so that base is read (before all else) and out written in whole rows of
+// 512 bytes. Bound by those.
 template <uint32_t kType>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterArgs a) {
   const AdapterRun run = a.run[blockIdx.z];
@@ -231,26 +251,37 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterArgs a) {
   if (r0 >= run.rows) return;
   const uint32_t rows = min(kUpRows, run.rows - r0);
   const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15, wave = threadIdx.x >> 6;
-  const uint32_t o0 = blockIdx.x * kUpOuts + 32 * wave;
-  __shared__ __attribute__((aligned(16))) float s_down[kUpRows][64 + 4];
-  float4_t acc[4][2] = {}, base[4][2];  // [row tile][output tile]
+  const uint32_t o0 = blockIdx.x * kUpOuts;
+  constexpr int kDownStride = 64 + 4, kOutStride = kUpOuts + 4;
+  __shared__ __attribute__((aligned(16))) float s_mem[kUpRows * kOutStride];  // A x, then the outputs
   const bool wide = a.outs % 4 == 0;
+  // This thread's pieces of four outputs.
+  constexpr int kPieces = kUpRows * kUpOuts / 4 / 256;
+  const uint32_t o = o0 + 4 * (threadIdx.x % (kUpOuts / 4)), row_of = threadIdx.x / (kUpOuts / 4);
+  constexpr uint32_t kRowStep = 256 / (kUpOuts / 4);
+  float4_t base[kPieces];
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int i = 0; i < kPieces; ++i) {
+    base[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const uint32_t row = row_of + kRowStep * i;
+    if (a.base == nullptr || row >= rows || o >= a.outs) continue;
+    const float* p = a.base + (uint64_t)(run.row0 + r0 + row) * a.outs + o;
+    if (wide) base[i] = *(const float4_t*)p;
+    else
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      base[t][n] = float4_t{0.f, 0.f, 0.f, 0.f};
-      const uint32_t row = 16 * t + c16, o = o0 + 16 * n + 4 * g;
-      if (a.base == nullptr || row >= rows || o >= a.outs) continue;
-      const float* p = a.base + (uint64_t)(run.row0 + r0 + row) * a.outs + o;
-      if (wide) base[t][n] = *(const float4_t*)p;
-      else
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e)
-          if (o + e < a.outs) base[t][n][e] = p[e];
-    }
+      for (uint32_t e = 0; e < 4; ++e)
+        if (o + e < a.outs) base[i][e] = p[e];
+  }
+  constexpr int kRowTiles = kUpRows / 16;
+  float4_t acc[kRowTiles][2] = {};  // [row tile][output tile]
   for (uint32_t rank0 = 0; rank0 < run.rank16; rank0 += 64) {
     const uint32_t ranks = min(64u, run.rank16 - rank0);
+    Raw<kType, 4> w[4][2];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        w[k][n].load(a.b, run.b_at + adapter_b_index(min(o0 + 32 * wave + 16 * n + c16, a.outs - 1), rank0 + min(16 * k, ranks - 16) + 4 * g, a.outs));
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < kUpRows * (ranks / 4); i += 256) {
       const uint32_t row = i / (ranks / 4), r = 4 * (i % (ranks / 4));
@@ -259,38 +290,40 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterArgs a) {
         const float* p = a.down + (uint64_t)(run.row0 + r0 + row) * a.splits * a.max_rank16 + rank0 + r;
         for (uint32_t s = 0; s < a.splits; ++s) sum += *(const float4_t*)(p + (uint64_t)s * a.max_rank16);
       }
-      *(float4_t*)&s_down[row][r] = sum * run.scale;
+      *(float4_t*)&s_mem[row * kDownStride + r] = sum * run.scale;
     }
     __syncthreads();
-    for (uint32_t r = 0; r < ranks; r += 16) {
-      Raw<kType, 4> w[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-        w[n].load(a.b, run.b_at + adapter_b_index(min(o0 + 16 * n + c16, a.outs - 1), rank0 + r + 4 * g, a.outs));
+    for (uint32_t k = 0; k < 4; ++k) {
+      if (16 * k >= ranks) break;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float4_t d = *(const float4_t*)&s_down[16 * t + c16][r + 4 * g];
+      for (int t = 0; t < kRowTiles; ++t) {
+        const float4_t d = *(const float4_t*)&s_mem[(16 * t + c16) * kDownStride + 16 * k + 4 * g];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int n = 0; n < 2; ++n) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[n][e], d[e], acc[t][n], 0, 0, 0);
+          for (int n = 0; n < 2; ++n) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[k][n][e], d[e], acc[t][n], 0, 0, 0);
       }
     }
   }
+  __syncthreads();
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < kRowTiles; ++t)
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const uint32_t row = 16 * t + c16, o = o0 + 16 * n + 4 * g;
-      if (row >= rows || o >= a.outs) continue;
-      float* p = a.out + (uint64_t)(run.row0 + r0 + row) * a.outs + o;
-      const float4_t y = base[t][n] + acc[t][n];
-      if (wide) *(float4_t*)p = y;
-      else
+    for (int n = 0; n < 2; ++n) *(float4_t*)&s_mem[(16 * t + c16) * kOutStride + 32 * wave + 16 * n + 4 * g] = acc[t][n];
+  __syncthreads();
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e)
-          if (o + e < a.outs) p[e] = y[e];
-    }
+  for (int i = 0; i < kPieces; ++i) {
+    const uint32_t row = row_of + kRowStep * i;
+    if (row >= rows || o >= a.outs) continue;
+    float* p = a.out + (uint64_t)(run.row0 + r0 + row) * a.outs + o;
+    const float4_t y = base[i] + *(const float4_t*)&s_mem[row * kOutStride + (o - o0)];
+    if (wide) *(float4_t*)p = y;
+    else
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e)
+        if (o + e < a.outs) p[e] = y[e];
+  }
 }
 
 // An adapter's weights into their stored form, the ranks behind its own zero.
@@ -341,7 +374,7 @@ hipError_t launch_adapter_long(const AdapterArgs& a, hipStream_t stream) {
   const dim3 up((a.outs + kUpOuts - 1) / kUpOuts, (a.max_rows + kUpRows - 1) / kUpRows, a.runs);
   return by_type(a.dtype, [&](auto type) {
     constexpr uint32_t kType = decltype(type)::value;
-    if (a.max_rank16) adapter_down_kernel<kType><<<down, 256, 0, stream>>>(a);
+    if (a.max_rank16) adapter_down_kernel<kType><<<down, 512, 0, stream>>>(a);
     adapter_up_kernel<kType><<<up, 256, 0, stream>>>(a);
     return hipGetLastError();
   });

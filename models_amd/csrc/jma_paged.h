@@ -135,7 +135,7 @@ constexpr uint32_t kSelectFloats = 8192;
 inline bool paged_supported(uint32_t d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 
 // Waves of an attention workgroup, and the slots one wave takes at a step.
-constexpr int paged_waves(int d) { return d >= 256 ? 4 : 8; }
+constexpr int paged_waves(int d) { return d >= 128 ? 4 : 8; }
 JMA_HD uint32_t paged_step(bool f16) { return f16 ? 32u : 16u; }
 
 // The steps (of paged_step slots) that a block of query rows at positions pos0 .. pos1 reads: all

@@ -571,7 +571,8 @@ __device__ __forceinline__ void store_token(const PagedView& kv, const PagedChun
 // output does its steps again, with those values taken out of the product and what they make of the
 // columns that see them (NaN) put in.
 template <typename KV, int D, bool kSelected, bool kFused>
-__global__ __launch_bounds__(64 * paged_waves(D)) void paged_attend_kernel(const PagedAttendArgs a) {
+__global__ __launch_bounds__(64 * paged_waves(D)) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D == 128 ? 2 : 1)))
+void paged_attend_kernel(const PagedAttendArgs a) {
   constexpr bool kF16 = std::is_same<KV, _Float16>::value;
   constexpr int kW = paged_waves(D), kNs = kF16 ? 8 : 4, kNv = D / 16;
   constexpr uint32_t kStep = kF16 ? 32 : 16, kThreads = 64 * kW;
