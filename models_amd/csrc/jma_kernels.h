@@ -331,8 +331,7 @@ hipError_t launch_qkgemm(const QMatArgs& a, uint32_t fmt, uint32_t shape, uint32
 // RoPE, norms and the store of the chunks' rows (a.num_heads 0 with no q_out), then the bounds of the
 // pages written where the cache keeps them.
 hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, hipStream_t stream);
-// max_pages: pages that the row furthest back sees.
-hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, uint32_t max_pages, hipStream_t stream);
+hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, hipStream_t stream);
 hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, hipStream_t stream);
 // Chunks of many rows over an f16 cache (no selected pages).
 hipError_t launch_paged_prefill(const PagedAttendArgs& a, uint32_t d, hipStream_t stream);

@@ -111,10 +111,13 @@ struct PagedSelectArgs {
   PagedRotation rot;
   uint32_t raw;
   uint32_t* pages;     // out: [rows][hkv][budget]
-  uint64_t* keys;      // scratch [row slot][hkv][key_stride]: the pages' scores as ordered integers
-  uint32_t* tickets;   // [row slot][hkv], zero between launches
+  float* keys;         // scratch [block][row of the block][2 key_stride]: scores in 32 bits, or in 64, as
+                       // ordered integers, where those are needed
+  float* maxima;       // scratch [block][max_wgs][4]: largest bound of a wave's pages
+  uint32_t* tickets;   // [block], zero between launches; block = (chunk, row block, kv head)
   uint32_t num_heads, group, top, first, last, budget;
-  uint32_t key_stride, max_rows;
+  uint32_t rows_per_block, max_blocks;  // query rows of a workgroup; row blocks of the chunk with the most
+  uint32_t key_stride, max_wgs;  // pages, and workgroups, of the row furthest back
   uint32_t chunks;
   PagedChunk c[kMaxChunks];
 };
@@ -129,6 +132,8 @@ struct PagedTableArgs {
 };
 static_assert(sizeof(PagedTableArgs) <= 4096, "kernel arguments exceed their limit");
 
+// Query rows of a selection workgroup: its matrix product has 16 columns.
+JMA_HD uint32_t select_rows(uint32_t group) { return group >= 16 ? 1u : 16u / group; }
 // Floats of a group's queries that the selection kernel stages where it takes them raw.
 constexpr uint32_t kSelectFloats = 8192;
 

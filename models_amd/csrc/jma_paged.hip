@@ -191,7 +191,6 @@ __device__ __forceinline__ uint64_t ordered(double x) {
   const uint64_t b = (uint64_t)__double_as_longlong(x == 0.0 ? 0.0 : x);
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
-
 // Sum over the 16 lanes of a row, in vector ALU exchanges; every lane gets the same bits.
 template <int kCtrl>
 __device__ __forceinline__ double row_moved(double x) {
@@ -208,265 +207,533 @@ __device__ __forceinline__ double row_sum(double x) {
   return x;
 }
 
-// The pages of one (row, kv head), ascending: the first `first`, the last `last` and the `top` others of
-// the largest keys, of equal ones the lowest. The key of the last page taken is narrowed by eight
-// bits a pass, from the highest bit in which any two keys differ, until every key that shares the bits
-// found so far is taken (two or three passes: the keys are spread). n > first + last + top.
-template <uint32_t kPickRounds>
-__device__ __forceinline__ void pick_pages(const uint64_t* keys, uint32_t n, uint32_t top, uint32_t first, uint32_t last,
-                                           uint32_t* out) {
-  __shared__ uint32_t s_hist[256], s_found[3], s_any[4][2], s_sum[4];
-  __shared__ uint32_t s_count[64];
-  constexpr uint32_t kPickPages = 256 * kPickRounds;  // keys the workgroup holds in registers
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint64_t k[kPickRounds];
-  auto candidate = [&](uint32_t p) JMA_INL { return p >= first && p + last < n; };
-  auto load = [&](uint32_t base) JMA_INL {
-#pragma unroll
-    for (uint32_t i = 0; i < kPickRounds; ++i) {
-      // Unconditional, so that all are in flight together: those of no candidate are not looked at.
-      const uint32_t p = min(base + 256 * i + tid, n - last - 1);
-      k[i] = __hip_atomic_load(&keys[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-  };
-  auto each = [&](auto&& f) JMA_INL {  // f(round's first page) over the keys, re-read where they are too many
-    for (uint32_t base = 0; base < n; base += kPickPages) {
-      if (n > kPickPages) load(base);
-      f(base);
-    }
-  };
-  load(0);
+template <int kCtrl>
+__device__ __forceinline__ float row_moved(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), kCtrl, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float max_wave(float x) {
+  x = fmaxf(x, row_moved<0x128>(x));
+  x = fmaxf(x, row_moved<0x124>(x));
+  x = fmaxf(x, row_moved<0x122>(x));
+  x = fmaxf(x, row_moved<0x121>(x));
+  return max_groups(x);
+}
 
-  // The bits in which the keys differ from the first one's.
-  const uint64_t reference = __hip_atomic_load(&keys[first], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  uint64_t differ = 0;
-  each([&](uint32_t base) JMA_INL {
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask, uint32_t lane) {
+  return (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+}
+
+// What picks a row's pages works on, in LDS: a wave's share.
+constexpr uint32_t kHeldScores = 1024, kPickBins = 512, kPickNear = 64;
+struct PickSpace {
+  uint32_t hist[4][kPickBins];
+  float score[4][kHeldScores];
+  uint32_t near[4][kPickNear];    // pages whose scores lie too near the border to be told apart in 32 bits
+  uint64_t exact[4][kPickNear];
+  float least[4], most[4];
+  uint32_t odd[4], sure[4], count[4];
+};
+
+// 64-bit keys of a row's candidates first <= p < end, at keys[p], read again in every pass.
+struct Keys {
+  const uint64_t* keys;
+  uint32_t first, end, lane;
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) {  // f(page, key, whether there is such a candidate)
+    for (uint32_t base = first; base < end; base += 256) {
+      uint64_t k[4];
 #pragma unroll
-    for (uint32_t i = 0; i < kPickRounds; ++i)
-      if (candidate(base + 256 * i + tid)) differ |= k[i] ^ reference;
+      for (uint32_t i = 0; i < 4; ++i)  // unconditional, so that all are in flight together
+        k[i] = __hip_atomic_load(&keys[min(base + 64 * i + lane, end - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) f(base + 64 * i + lane, k[i], base + 64 * i + lane < end);
+    }
+  }
+};
+
+// Which of the bins of a histogram holds the need-th largest; then need is its rank within the bin.
+template <uint32_t kPerLane>
+__device__ __forceinline__ void border_bin(const uint32_t* hist, uint32_t lane, uint32_t& need, uint32_t& bin, uint32_t& count) {
+  uint32_t c[kPerLane], mine = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kPerLane; ++i) c[i] = hist[kPerLane * lane + i], mine += c[i];
+  uint32_t above = mine;
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    const uint32_t x = __shfl_down(above, m);
+    if (lane + m < 64) above += x;
+  }
+  uint32_t left = above - mine, b = 0, n = 0, rest = 0;  // entries of the bins above this lane's
+  bool found = false;
+#pragma unroll
+  for (int i = (int)kPerLane - 1; i >= 0; --i) {
+    if (!found && left + c[i] >= need && left < need) {
+      found = true;
+      b = kPerLane * lane + i;
+      n = c[i];
+      rest = need - left;
+    }
+    left += c[i];
+  }
+  const int at = __ffsll((long long)__ballot(found)) - 1;
+  bin = __builtin_amdgcn_readlane(b, at);
+  count = __builtin_amdgcn_readlane(n, at);
+  need = __builtin_amdgcn_readlane(rest, at);
+}
+
+// The n-th largest of 64-bit keys: eight bits a pass, from the highest bit in which any two differ, until all
+// keys that share the bits found are among the n largest.
+__device__ __forceinline__ uint64_t nth_largest(Keys& keys, uint32_t n, uint32_t* hist) {
+  const uint32_t lane = keys.lane;
+  const uint64_t reference = __hip_atomic_load(&keys.keys[keys.first], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  uint32_t lo = 0, hi = 0;
+  keys.each([&](uint32_t, uint64_t x, bool there) JMA_INL {
+    if (!there) return;
+    lo |= (uint32_t)(x ^ reference);
+    hi |= (uint32_t)((x ^ reference) >> 32);
   });
-  uint32_t lo = (uint32_t)differ, hi = (uint32_t)(differ >> 32);
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) {
     lo |= __shfl_xor(lo, m);
     hi |= __shfl_xor(hi, m);
   }
-  if (lane == 0) s_any[wave][0] = lo, s_any[wave][1] = hi;
-  __syncthreads();
-  differ = (uint64_t)(s_any[0][1] | s_any[1][1] | s_any[2][1] | s_any[3][1]) << 32 | (s_any[0][0] | s_any[1][0] | s_any[2][0] | s_any[3][0]);
-  int shift = differ == 0 ? 0 : max(0, 64 - __clzll((long long)differ) - 8);
-  uint64_t prefix = shift + 8 >= 64 ? 0 : reference >> (shift + 8);  // bits found so far
-  uint32_t need = top;
-  bool all = top == 0 || differ == 0;
-  if (differ == 0) prefix = reference;
-  const bool tie = differ == 0;  // one key throughout: the lowest pages
-  for (; !all; shift = max(0, shift - 8)) {
-    s_hist[tid] = 0;
-    __syncthreads();
-    each([&](uint32_t base) JMA_INL {
+  int shift = hi ? 64 - __clz(hi) : lo ? 32 - __clz(lo) : 0;  // the bits in which keys differ
+  if (shift == 0) return reference;
+  uint64_t prefix = shift >= 64 ? 0 : reference >> shift;
+  uint32_t need = n;
+  while (shift > 0) {
+    const int bits = min(8, shift), next = shift - bits;
 #pragma unroll
-      for (uint32_t i = 0; i < kPickRounds; ++i)
-        if (candidate(base + 256 * i + tid) && (shift + 8 >= 64 || k[i] >> (shift + 8) == prefix))
-          atomicAdd(&s_hist[(k[i] >> shift) & 255], 1u);
+    for (int i = 0; i < 4; ++i) hist[64 * i + lane] = 0;
+    __builtin_amdgcn_wave_barrier();
+    keys.each([&](uint32_t, uint64_t x, bool there) JMA_INL {
+      if (there && (shift >= 64 || x >> shift == prefix)) atomicAdd(&hist[(uint32_t)(x >> next) & ((1u << bits) - 1)], 1u);
     });
-    __syncthreads();
-    // How many keys are in bin `tid` and above.
-    const uint32_t mine = s_hist[tid];
-    uint32_t above = mine;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-      const uint32_t x = __shfl_down(above, m);
-      if (lane + m < 64) above += x;
-    }
-    if (lane == 0) s_sum[wave] = above;
-    __syncthreads();
-    for (uint32_t w = wave + 1; w < 4; ++w) above += s_sum[w];
-    if (above >= need && above - mine < need) {
-      s_found[0] = tid;
-      s_found[1] = need - (above - mine);
-      s_found[2] = mine;
-    }
-    __syncthreads();
-    prefix = prefix << 8 | s_found[0];
-    need = s_found[1];
-    all = need == s_found[2] || shift == 0;
-    if (all) break;
-    if (shift < 8) {  // the last pass takes the bits that are left
-      const int left = shift;
-      s_hist[tid] = 0;
-      __syncthreads();
-      each([&](uint32_t base) JMA_INL {
-#pragma unroll
-        for (uint32_t i = 0; i < kPickRounds; ++i)
-          if (candidate(base + 256 * i + tid) && k[i] >> left == prefix) atomicAdd(&s_hist[k[i] & ((1u << left) - 1)], 1u);
-      });
-      __syncthreads();
-      const uint32_t bin = s_hist[tid];
-      uint32_t up = bin;
-#pragma unroll
-      for (int m = 1; m < 64; m *= 2) {
-        const uint32_t x = __shfl_down(up, m);
-        if (lane + m < 64) up += x;
-      }
-      if (lane == 0) s_sum[wave] = up;
-      __syncthreads();
-      for (uint32_t w = wave + 1; w < 4; ++w) up += s_sum[w];
-      if (up >= need && up - bin < need) {
-        s_found[0] = tid;
-        s_found[1] = need - (up - bin);
-        s_found[2] = bin;
-      }
-      __syncthreads();
-      prefix = prefix << left | s_found[0];
-      need = s_found[1];
-      shift = 0;
-      break;
-    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    uint32_t bin, count;
+    border_bin<4>(hist, lane, need, bin, count);
+    prefix = shift >= 64 ? (uint64_t)bin : prefix << bits | bin;
+    shift = next;
+    if (need == count) break;
   }
-  // Taken: keys above the last one's bits, and of those that share them the lowest `need` pages (all of
-  // them unless keys are equal).
-  uint32_t taken = 0, equal = 0;  // before this round of kPickPages pages
-  each([&](uint32_t base) JMA_INL {
-    uint32_t flags = 0, ties = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kPickRounds; ++i) {
-      const uint32_t p = base + 256 * i + tid;
-      const uint64_t x = tie ? k[i] : k[i] >> shift;
-      const bool c = candidate(p), eq = c && top != 0 && x == prefix;
-      if (p < n && (!c || (top != 0 && x > prefix))) flags |= 1u << i;
-      if (eq) ties |= 1u << i;
-    }
-    // Ranks of the equal keys, in page order.
-    auto ranks = [&](uint32_t set, uint32_t before, uint32_t* total) JMA_INL {
-      __syncthreads();
-#pragma unroll
-      for (uint32_t i = 0; i < kPickRounds; ++i) {
-        const uint64_t b = __ballot((set >> i) & 1);
-        if (lane == 0) s_count[4 * i + wave] = __popcll(b);
-      }
-      __syncthreads();
-      if (wave == 0) {
-        const uint32_t mine = lane < 4 * kPickRounds ? s_count[lane] : 0;
-        uint32_t sum = mine;
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) {
-          const uint32_t x = __shfl_up(sum, m);
-          if (lane >= (uint32_t)m) sum += x;
-        }
-        s_count[lane] = sum - mine;
-        if (lane == 63) s_sum[0] = sum;
-      }
-      __syncthreads();
-      *total = before + s_sum[0];
-      return before;
-    };
-    auto rank = [&](uint32_t set, uint32_t i, uint32_t before) JMA_INL {
-      const uint64_t b = __ballot((set >> i) & 1);
-      return before + s_count[4 * i + wave] + (uint32_t)__popcll(b & ((1ull << lane) - 1));
-    };
-    uint32_t next;
-    const uint32_t before_eq = ranks(ties, equal, &next);
-#pragma unroll
-    for (uint32_t i = 0; i < kPickRounds; ++i) {
-      const uint32_t r = rank(ties, i, before_eq);
-      if (((ties >> i) & 1) && r < need) flags |= 1u << i;
-    }
-    equal = next;
-    const uint32_t before = ranks(flags, taken, &next);
-#pragma unroll
-    for (uint32_t i = 0; i < kPickRounds; ++i) {
-      const uint32_t r = rank(flags, i, before);
-      if ((flags >> i) & 1) out[r] = base + 256 * i + tid;
-    }
-    taken = next;
+  if (shift == 0) return prefix;
+  // All keys with these bits are taken: the smallest of them.
+  uint64_t least = ~0ull;
+  keys.each([&](uint32_t, uint64_t x, bool there) JMA_INL {
+    if (there && x >> shift == prefix) least = x < least ? x : least;
   });
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    const uint64_t x = __shfl_xor(least, m);
+    least = x < least ? x : least;
+  }
+  return least;
 }
 
-// Workgroup = (64 pages, row x kv head, chunk). Scores: for a page with bounds lo, hi and each query
-// head of the group, sum_d max(q_d lo_d, q_d hi_d), which no key of the page exceeds; the page's score
-// is the largest of the heads'. The sums are formed in 64 bits, where the products are exact, so that
-// which of two nearly equal pages is taken does not depend on the order of a sum. 16 lanes take a page,
-// four pages each, whose table entries and bounds are all in flight before the first is used: the
-// kernel's time is those two memory round trips and the pick's, not its arithmetic (64 pages, 4 heads of
-// 128: 1 us). The last workgroup of a (row, kv head) to finish picks the pages.
+// Workgroup = (64 pages, block of query rows x kv head, chunk). A page with bounds lo, hi scores
+// sum_d max(q_d lo_d, q_d hi_d) for a query head, which no key of the page exceeds, and the largest of the
+// heads' for a (row, kv head). That is the product of [lo, hi] with [min(q, 0), max(q, 0)]: 16 pages x 16
+// columns (rows x heads) a matrix product, in 32 bits (f16 bounds: q as two halves, like the attention's).
+//
+// Which of two nearly equal pages is taken must not depend on a rounding. The 32-bit scores are off by at
+// most eps = (2^-22 + (4 d + 16) 2^-23) |q|_1 max|bound|; with T the border score, pages above T + 2 eps are
+// taken and pages below T - 2 eps are not, whatever the exact scores are, and the few between are scored
+// again in 64 bits, where the products are exact (one or two of a thousand pages). Where they are more
+// than 64, or a bound is infinite, all pages of the row are.
+//
+// 16 pages' table entries and bounds are in flight before the first is used: the kernel's time is those
+// two memory round trips, the keys' way to the last workgroup of the block to finish, and its pick (a wave
+// a row). Scored in 64 bits throughout it took 45 us for 61 rows of 12 heads of 128 over 626 pages,
+// SELECT_FIGURES.
 template <typename KV, int D>
 __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs a) {
+  constexpr bool kF16 = std::is_same<KV, _Float16>::value;
+  constexpr int kQStride = D + 4;
   const PagedChunk c = a.c[blockIdx.z];
-  const uint32_t hkv = a.kv.hkv, kvh = blockIdx.y % hkv, r = blockIdx.y / hkv;
-  if (r >= c.rows) return;
-  const uint32_t pos = c.start + r, row = c.row0 + r;
-  const uint32_t n = (pos >> a.kv.page_log2) + 1;
-  const uint32_t first_page = blockIdx.x * kSelectPages;
-  if (first_page >= n) return;
-  const uint32_t wgs = (n + kSelectPages - 1) / kSelectPages;
-  uint32_t* out = a.pages + ((uint64_t)row * hkv + kvh) * a.budget;
-  if (n <= a.budget) {  // every page
-    if (blockIdx.x == 0)
-      for (uint32_t i = threadIdx.x; i < a.budget; i += 256) out[i] = i < n ? i : kNoPage;
-    return;
-  }
-  const uint64_t slot = ((uint64_t)blockIdx.z * a.max_rows + r) * hkv + kvh;
-  uint64_t* keys = a.keys + slot * a.key_stride;
-  extern __shared__ __attribute__((aligned(16))) float s_queries[];  // raw: [group][D + 4]
-  __shared__ float s_scale[kSelectFloats / 32];
+  const uint32_t hkv = a.kv.hkv, kvh = blockIdx.y % hkv, r0 = blockIdx.y / hkv * a.rows_per_block;
+  if (r0 >= c.rows) return;
+  const uint32_t rows = min(a.rows_per_block, c.rows - r0);
+  const uint32_t pos0 = c.start + r0, row0 = c.row0 + r0;
+  auto pages_of = [&](uint32_t r) JMA_INL { return ((pos0 + r) >> a.kv.page_log2) + 1; };
+  const uint32_t n1 = pages_of(rows - 1), first_page = blockIdx.x * kSelectPages;
+  if (first_page >= n1) return;
+  auto list_of = [&](uint32_t r) JMA_INL { return a.pages + ((uint64_t)(row0 + r) * hkv + kvh) * a.budget; };
+  if (blockIdx.x == 0)  // rows that see no more pages than they may
+    for (uint32_t r = 0; r < rows && pages_of(r) <= a.budget; ++r)
+      for (uint32_t i = threadIdx.x; i < a.budget; i += 256) list_of(r)[i] = i < pages_of(r) ? i : kNoPage;
+  if (n1 <= a.budget) return;
+  const uint32_t wgs = (n1 + kSelectPages - 1) / kSelectPages;
+  const uint64_t block = ((uint64_t)blockIdx.z * a.max_blocks + blockIdx.y / hkv) * hkv + kvh;
+  float* keys = a.keys + block * a.rows_per_block * 2 * a.key_stride;  // [row][2 key_stride]
+  float* maxima = a.maxima + block * 4 * a.max_wgs;
 
-  constexpr int kE = D / 16, kP = kSelectPages / 16;
-  typedef KV kve_t __attribute__((ext_vector_type(kE)));
-  const uint32_t lane16 = threadIdx.x % 16, own = threadIdx.x / 16;
+  extern __shared__ __attribute__((aligned(16))) float s_queries[];  // raw: [group][D + 4]
+  union Space {
+    struct {
+      float q[16 * kQStride], score[kSelectPages][17], max[4];
+    };
+    PickSpace pick;
+  };
+  __shared__ __attribute__((aligned(16))) Space s_mem;
+  __shared__ float s_l1[16], s_scale[kSelectFloats / 32];
+  __shared__ uint32_t s_last;
+  float* const s_q = s_mem.q;
+  PickSpace& space = s_mem.pick;
+
+  const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c16 = lane & 15;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t* table = a.kv.table + (uint64_t)c.seq * a.kv.table_stride;
-  uint32_t page[kP];
+  auto bounds_of = [&](uint32_t p) JMA_INL { return (const KV*)a.kv.bounds + ((uint64_t)table[p] * hkv + kvh) * 2 * D; };
+
+  // This lane's share of 16 pages' bounds: page 16 wave + c16.
+  constexpr int kCh = kF16 ? D / 32 : D / 16;  // operands of either bound
+  typedef std::conditional_t<kF16, half8_t, float4_t> operand_t;
+  constexpr int kE = kF16 ? 8 : 4;
+  operand_t lo[kCh], hi[kCh];
+  {
+    const KV* b = bounds_of(min(first_page + 16 * wave + c16, n1 - 1)) + kE * g;
 #pragma unroll
-  for (int i = 0; i < kP; ++i) page[i] = table[min(first_page + 16 * i + own, n - 1)];
-  kve_t lo[kP], hi[kP];
-#pragma unroll
-  for (int i = 0; i < kP; ++i) {
-    const KV* b = (const KV*)a.kv.bounds + ((uint64_t)page[i] * hkv + kvh) * 2 * D + lane16 * kE;
-    lo[i] = *(const kve_t*)b;
-    hi[i] = *(const kve_t*)(b + D);
-  }
-  const float* q = a.q + ((uint64_t)row * a.num_heads + kvh * a.group) * D;
-  if (a.raw) {
-    for (uint32_t i = threadIdx.x; i < a.group * (D / 4); i += 256)
-      *(float4_t*)&s_queries[i / (D / 4) * (D + 4) + 4 * (i % (D / 4))] = *(const float4_t*)(q + 4 * i);
-    prepare_token<D, D + 4>(s_queries, s_scale, a.group, 0, false, a.rot, pos, 256);
-  }
-  double best[kP];
-  bool odd[kP];
-#pragma unroll
-  for (int i = 0; i < kP; ++i) best[i] = -INFINITY, odd[i] = false;
-  for (uint32_t h = 0; h < a.group; ++h) {
-    float x[kE];
-#pragma unroll
-    for (int e = 0; e < kE; ++e) x[e] = a.raw ? s_queries[h * (D + 4) + lane16 * kE + e] : q[(uint64_t)h * D + lane16 * kE + e];
-#pragma unroll
-    for (int i = 0; i < kP; ++i) {
-      double s = 0.0;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) s = fma((double)x[e], (double)(float)(x[e] >= 0.0f ? hi[i][e] : lo[i][e]), s);
-      s = row_sum(s);
-      odd[i] = odd[i] || s != s;
-      best[i] = s > best[i] ? s : best[i];
+    for (int i = 0; i < kCh; ++i) {
+      lo[i] = *(const operand_t*)(b + 4 * kE * i);
+      hi[i] = *(const operand_t*)(b + D + 4 * kE * i);
     }
   }
-#pragma unroll
-  for (int i = 0; i < kP; ++i) {
-    const uint32_t p = first_page + 16 * i + own;
-    if (lane16 == 0 && p < n)
-      __hip_atomic_store(&keys[p], odd[i] ? 0xFFFFFFFFFFFFFFFFull : ordered(best[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const float* q = a.q + ((uint64_t)row0 * a.num_heads + kvh * a.group) * D;
+  if (a.raw) {
+    for (uint32_t i = tid; i < a.group * (D / 4); i += 256)
+      *(float4_t*)&s_queries[i / (D / 4) * kQStride + 4 * (i % (D / 4))] = *(const float4_t*)(q + 4 * i);
+    prepare_token<D, kQStride>(s_queries, s_scale, a.group, 0, false, a.rot, pos0, 256);
   }
+  auto query = [&](uint32_t r, uint32_t h) JMA_INL -> const float* {
+    return a.raw ? s_queries + h * kQStride : q + ((uint64_t)r * a.num_heads + h) * D;
+  };
+  for (uint32_t h0 = 0; h0 < a.group; h0 += 16) {
+    const uint32_t heads = min(16u, a.group - h0);
+    __syncthreads();
+    for (uint32_t i = tid; i < 16 * (D / 4); i += 256) {
+      const uint32_t col = i / (D / 4), e = 4 * (i % (D / 4)), r = col / heads;
+      float4_t x = {0.f, 0.f, 0.f, 0.f};
+      if (r < rows) x = *(const float4_t*)(query(r, h0 + col % heads) + e);
+      *(float4_t*)&s_q[col * kQStride + e] = x;
+    }
+    __syncthreads();
+    float factor = 1.0f, l1 = 0.0f;
+    float4_t s = {0.f, 0.f, 0.f, 0.f};
+    const float* mine = s_q + c16 * kQStride + kE * g;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kCh; ++i)
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const float x = fabsf(mine[4 * kE * i + e]);
+        l1 += x;
+        top = fmaxf(top, x);
+      }
+    l1 = sum_groups(l1);
+    if constexpr (kF16) {
+      top = max_groups(top);
+      int ex = 0;
+      if (top > 0.0f && top < INFINITY) ex = __builtin_amdgcn_frexp_expf(top);
+      ex = max(ex, -100);
+      factor = __builtin_amdgcn_ldexpf(1.0f, ex - 14);
+#pragma unroll
+      for (int i = 0; i < kCh; ++i) {
+        half8_t below_h, below_l, above_h, above_l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_amdgcn_ldexpf(mine[32 * i + e], 14 - ex);
+          _Float16 h, l;
+          halves(fminf(x, 0.0f), h, l);
+          below_h[e] = h;
+          below_l[e] = l;
+          halves(fmaxf(x, 0.0f), h, l);
+          above_h[e] = h;
+          above_l[e] = l;
+        }
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[i], below_l, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[i], above_l, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[i], below_h, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[i], above_h, s, 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCh; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = mine[16 * i + e];
+          s = __builtin_amdgcn_mfma_f32_16x16x4f32(lo[i][e], fminf(x, 0.0f), s, 0, 0, 0);
+          s = __builtin_amdgcn_mfma_f32_16x16x4f32(hi[i][e], fmaxf(x, 0.0f), s, 0, 0, 0);
+        }
+    }
+    // Lane (g, c) holds pages 4g .. 4g + 3 of column c. A score that is not finite stays so.
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_mem.score[16 * wave + 4 * g + i][c16] = s[i] * factor;
+    l1 = l1 < INFINITY ? l1 : INFINITY;  // also where it is no number
+    if (wave == 0 && g == 0) s_l1[c16] = h0 == 0 ? l1 : fmaxf(l1, s_l1[c16]);
+    __syncthreads();
+    for (uint32_t i = tid; i < kSelectPages * rows; i += 256) {
+      const uint32_t p = first_page + i % kSelectPages, r = i / kSelectPages;
+      float best = -INFINITY;
+      bool odd = false;
+      for (uint32_t h = 0; h < heads; ++h) {
+        const float x = s_mem.score[i % kSelectPages][r * heads + h];
+        odd = odd || !(fabsf(x) < INFINITY);
+        best = fmaxf(best, x);
+      }
+      if (p >= n1) continue;
+      float* key = keys + (uint64_t)r * 2 * a.key_stride + p;
+      if (h0 > 0) {
+        const float x = __hip_atomic_load(key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        odd = odd || x != x;
+        best = fmaxf(best, x);
+      }
+      __hip_atomic_store(key, odd ? NAN : best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kCh; ++i)
+#pragma unroll
+    for (int e = 0; e < kE; ++e) most = fmaxf(most, fmaxf(fabsf((float)lo[i][e]), fabsf((float)hi[i][e])));
+  most = max_wave(most);
+  if (lane == 0) __hip_atomic_store(&maxima[4 * blockIdx.x + wave], most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // The keys are acknowledged (visible device-wide) before the ticket is taken.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (wgs > 1) {
-    __shared__ uint32_t s_last;
-    if (threadIdx.x == 0)
-      s_last = __hip_atomic_fetch_add(&a.tickets[slot], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) s_last = __hip_atomic_fetch_add(&a.tickets[block], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (s_last + 1 != wgs) return;
-    if (threadIdx.x == 0) __hip_atomic_store(&a.tickets[slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) __hip_atomic_store(&a.tickets[block], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  if (n <= 1024) pick_pages<4>(keys, n, a.top, a.first, a.last, out);
-  else pick_pages<16>(keys, n, a.top, a.first, a.last, out);
+
+  // Exact score of page p, of the 16 lanes that call with it.
+  auto exact = [&](uint32_t r, uint32_t p) JMA_INL -> uint64_t {
+    constexpr int kX = D / 16;
+    const KV* b = bounds_of(p) + c16 * kX;
+    double best = -INFINITY;
+    bool odd = false;
+    for (uint32_t h = 0; h < a.group; ++h) {
+      const float* x = query(r, h) + c16 * kX;
+      double s = 0.0;
+#pragma unroll
+      for (int e = 0; e < kX; ++e) {
+        const float low = (float)b[e], high = (float)b[D + e];
+        s = fma((double)x[e], (double)(x[e] > 0.0f ? high : low), s);
+        if (x[e] == 0.0f) s = fma((double)x[e], (double)high, s);  // either infinity against a zero counts
+      }
+      s = row_sum(s);
+      odd = odd || s != s;
+      best = s > best ? s : best;
+    }
+    return odd ? 0xFFFFFFFFFFFFFFFFull : ordered(best);
+  };
+  // The pages of row r, by a wave of its own, or by all four.
+  auto pick = [&](uint32_t r, auto team) JMA_INL {
+    constexpr uint32_t kWaves = decltype(team)::value, kBins = kWaves * kPickBins;
+    const uint32_t m = kWaves == 1 ? 0 : wave, w = wave - m;  // which of the team; its first wave, whose share of the LDS it has
+    auto meet = [&]() JMA_INL {
+      if constexpr (kWaves > 1) {
+        __syncthreads();
+      } else {
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+    };
+    const uint32_t n = pages_of(r);
+    uint32_t* out = list_of(r);
+    if (m == 0) {
+      for (uint32_t i = lane; i < a.first; i += 64) out[i] = i;
+      for (uint32_t i = lane; i < a.last; i += 64) out[a.first + a.top + i] = n - a.last + i;
+    }
+    if (a.top == 0) return;
+    out += a.first;
+    float* row_keys = keys + (uint64_t)r * 2 * a.key_stride;
+    // This wave's share of the candidates, kept in LDS where it fits.
+    const uint32_t candidates = n - a.last - a.first, share = (candidates + 64 * kWaves - 1) / (64 * kWaves) * 64;
+    const uint32_t p0 = a.first + min(m * share, candidates), p1 = a.first + min((m + 1) * share, candidates);
+    const bool held = share <= kHeldScores;
+    float* mine = space.score[wave];
+    uint32_t* hist = space.hist[w];
+    float bound = 0.0f;  // the largest of the pages' bounds
+    for (uint32_t i = lane; i < 4 * wgs; i += 64) bound = fmaxf(bound, __hip_atomic_load(&maxima[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+#pragma unroll
+    for (uint32_t i = 0; i < kPickBins / 64; ++i) hist[kPickBins * m + 64 * i + lane] = 0;
+    float least = INFINITY, most = -INFINITY;
+    bool odd = false;
+    for (uint32_t b = p0; b < p1; b += 512) {
+      float x[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i)  // unconditional, so that all are in flight together
+        x[i] = __hip_atomic_load(&row_keys[min(b + 64 * i + lane, p1 - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {  // the last one again does no harm
+        odd = odd || x[i] != x[i];
+        least = fminf(least, x[i]);
+        most = fmaxf(most, x[i]);
+        if (held) mine[b - p0 + 64 * i + lane] = x[i];
+      }
+    }
+    auto each = [&](auto&& f) JMA_INL {  // f(page, score, whether there is such a candidate)
+      for (uint32_t b = p0; b < p1; b += 256) {
+        float x[4];
+        if (held) {
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) x[i] = mine[b - p0 + 64 * i + lane];
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i)
+            x[i] = __hip_atomic_load(&row_keys[min(b + 64 * i + lane, p1 - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) f(b + 64 * i + lane, x[i], b + 64 * i + lane < p1);
+      }
+    };
+    bound = max_wave(bound);
+    least = -max_wave(-least);
+    most = max_wave(most);
+    uint32_t odds = __ballot(odd) != 0 ? 1 : 0;
+    if constexpr (kWaves > 1) {
+      if (lane == 0) space.least[wave] = least, space.most[wave] = most, space.odd[wave] = odds;
+      meet();
+#pragma unroll
+      for (uint32_t i = 0; i < kWaves; ++i) {
+        least = fminf(least, space.least[i]);
+        most = fmaxf(most, space.most[i]);
+        odds |= space.odd[i];
+      }
+    } else {
+      meet();
+    }
+    const uint32_t heads = min(16u, a.group);
+    float l1 = 0.0f;
+    for (uint32_t h = 0; h < heads; ++h) l1 = fmaxf(l1, s_l1[r * heads + h]);
+    const float eps = 1.001f * (0x1p-22f + (4 * D + 16) * 0x1p-23f) * l1 * bound + 0x1p-120f;  // and underflows
+    // Everything is scored in 64 bits where a score, or the steps of the histogram, are out of range.
+    const bool all = odds != 0 || !(l1 < INFINITY) || !(eps < INFINITY) || !(most - least > 0x1p-90f && most - least < INFINITY);
+    const float steps = (float)(kBins - 1) / (most - least), off = 2.0f * eps;
+    auto bin_of = [&](float x) JMA_INL { return min((uint32_t)fmaxf((x - least) * steps, 0.0f), kBins - 1); };
+    uint32_t bin = 0;
+    if (!all) {
+      each([&](uint32_t, float x, bool there) JMA_INL {
+        if (there) atomicAdd(&hist[bin_of(x)], 1u);
+      });
+      meet();
+      uint32_t need = a.top, count;
+      border_bin<kBins / 64>(hist, lane, need, bin, count);
+    }
+    auto above = [&](float x) JMA_INL { return !all && bin_of(x - off) > bin; };
+    auto near = [&](float x) JMA_INL { return all || (bin_of(x - off) <= bin && bin_of(x + off) >= bin); };
+    uint32_t sure = 0, count = 0;
+    if (!all) {
+      each([&](uint32_t p, float x, bool there) JMA_INL {
+        sure += (uint32_t)__popcll(__ballot(there && above(x)));
+        const bool in = there && near(x);
+        const uint64_t b = __ballot(in);
+        const uint32_t i = count + lanes_below(b, lane);
+        if (in && i < kPickNear) space.near[wave][i] = p;
+        count += (uint32_t)__popcll(b);
+      });
+      if constexpr (kWaves > 1)
+        if (lane == 0) space.sure[wave] = sure, space.count[wave] = count;
+      meet();
+    }
+    // Of the whole row, and of the waves before this one.
+    uint32_t all_sure = sure, all_near = count, near_before = 0, sure_before = 0, start[kWaves + 1] = {};
+    if constexpr (kWaves > 1) {
+      all_sure = all_near = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < kWaves; ++i) {
+        if (i == m) sure_before = all_sure, near_before = all_near;
+        start[i] = all_near;
+        all_sure += space.sure[i];
+        all_near += space.count[i];
+      }
+    }
+    if (!all && (all_near <= kPickNear || all_sure + all_near == a.top)) {
+      uint64_t taken = ~0ull;  // of those near
+      if (all_sure + all_near != a.top) {
+        for (uint32_t b = 4 * m; b < all_near; b += 4 * kWaves) {
+          uint32_t i = min(b + g, all_near - 1), of = w;
+          if constexpr (kWaves > 1) {
+#pragma unroll
+            for (uint32_t k = 1; k < kWaves; ++k)
+              if (i >= start[k]) of = k;
+            i -= start[0] * (of == 0) + start[1] * (of == 1) + start[2] * (of == 2) + start[3] * (of == 3);
+          }
+          const uint64_t e = exact(r, space.near[of][i]);
+          if (c16 == 0 && b + g < all_near) space.exact[w][b + g] = e;
+        }
+        meet();
+        const uint64_t e = space.exact[w][min(lane, all_near - 1)];
+        uint32_t better = 0;
+        for (uint32_t i = 0; i < all_near; ++i) {
+          const uint64_t x = space.exact[w][i];
+          better += x > e || (x == e && i < lane) ? 1u : 0u;
+        }
+        taken = __ballot(lane < all_near && better < a.top - all_sure);
+      }
+      uint32_t seen = near_before;
+      uint32_t at = sure_before + (taken == ~0ull ? near_before : (uint32_t)__popcll(taken & ((near_before < 64 ? 1ull << near_before : 0ull) - 1)));
+      each([&](uint32_t p, float x, bool there) JMA_INL {
+        const bool in = there && near(x);
+        const uint64_t b = __ballot(in);
+        const uint32_t i = seen + lanes_below(b, lane);
+        const bool take = (there && above(x)) || (in && (taken == ~0ull || ((taken >> (i & 63)) & 1)));
+        seen += (uint32_t)__popcll(b);
+        const uint64_t t = __ballot(take);
+        if (take) out[at + lanes_below(t, lane)] = p;
+        at += (uint32_t)__popcll(t);
+      });
+      return;
+    }
+    // Keys of 64 bits for all that are near, over the scores: whose place is first read by every wave.
+    meet();
+    uint64_t* wide = (uint64_t*)row_keys;
+    if (m != 0) return;
+    Keys k{wide, a.first, a.first + candidates, lane};
+    // From the last page to the first: key p lies over scores 2p and 2p + 1.
+    for (uint32_t left = candidates; left > 0;) {
+      const uint32_t len = (left - 1) % 64 + 1, b = k.first + left - len;
+      const float v = __hip_atomic_load(&row_keys[min(b + lane, k.end - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const bool there = lane < len;
+      uint64_t in = __ballot(there && near(v));
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (there && !near(v)) __hip_atomic_store(&wide[b + lane], above(v) ? ~0ull : 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      while (in != 0) {
+        uint32_t at[4];
+        uint32_t found = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          at[i] = in != 0 ? (uint32_t)__ffsll((long long)in) - 1 : at[i > 0 ? i - 1 : 0];
+          if (in != 0) ++found, in &= in - 1;
+        }
+        const uint32_t p = b + (g == 0 ? at[0] : g == 1 ? at[1] : g == 2 ? at[2] : at[3]);
+        const uint64_t e = exact(r, p);
+        if (c16 == 0 && g < found) __hip_atomic_store(&wide[p], e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      left -= len;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint64_t border = nth_largest(k, a.top, space.hist[w]);
+    uint32_t larger = 0;
+    k.each([&](uint32_t, uint64_t x, bool there) JMA_INL { larger += (uint32_t)__popcll(__ballot(there && x > border)); });
+    uint32_t at = 0, equal = 0;
+    k.each([&](uint32_t p, uint64_t x, bool there) JMA_INL {
+      const uint64_t b = __ballot(there && x == border);
+      const bool take = there && (x > border || (x == border && equal + lanes_below(b, lane) < a.top - larger));
+      equal += (uint32_t)__popcll(b);
+      const uint64_t t = __ballot(take);
+      if (take) out[at + lanes_below(t, lane)] = p;
+      at += (uint32_t)__popcll(t);
+    });
+  };
+  if (rows == 1)
+    pick(0, std::integral_constant<uint32_t, 4>{});
+  else
+    for (uint32_t r = wave; r < rows; r += 4)
+      if (pages_of(r) > a.budget) pick(r, std::integral_constant<uint32_t, 1>{});
 }
 
 // ================================================================ attention
@@ -1032,13 +1299,12 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, h
   });
 }
 
-hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, uint32_t max_pages, hipStream_t stream) {
+hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, hipStream_t stream) {
   return by_shape(f16, d, [&](auto kv, auto dim) {
     using KV = decltype(kv);
     constexpr int D = decltype(dim)::value;
-    const uint32_t wgs = (max_pages + kSelectPages - 1) / kSelectPages;
     const uint32_t lds = a.raw ? a.group * (D + 4) * 4 : 0;
-    paged_select_kernel<KV, D><<<dim3(wgs, a.max_rows * a.kv.hkv, a.chunks), 256, lds, stream>>>(a);
+    paged_select_kernel<KV, D><<<dim3(a.max_wgs, a.max_blocks * a.kv.hkv, a.chunks), 256, lds, stream>>>(a);
     return hipGetLastError();
   });
 }

@@ -335,19 +335,22 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, h
   });
 }
 
-hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, uint32_t max_pages, hipStream_t stream) {
-  return run(stream, "paged_select_kernel", [a, f16, d, max_pages] {
-    check_grid((max_pages + kSelectPages - 1) / kSelectPages, (uint64_t)a.max_rows * a.kv.hkv, a.chunks);
-    check(a.keys, (uint64_t)a.chunks * a.max_rows * a.kv.hkv * a.key_stride * 8, "page scores");
-    check(a.tickets, (uint64_t)a.chunks * a.max_rows * a.kv.hkv * 4, "tickets");
-    for (uint64_t i = 0; i < (uint64_t)a.chunks * a.max_rows * a.kv.hkv; ++i)
+hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, hipStream_t stream) {
+  return run(stream, "paged_select_kernel", [a, f16, d] {
+    check_grid(a.max_wgs, (uint64_t)a.max_blocks * a.kv.hkv, a.chunks);
+    const uint64_t blocks = (uint64_t)a.chunks * a.max_blocks * a.kv.hkv;
+    check(a.keys, blocks * a.rows_per_block * 2 * a.key_stride * 4, "page scores");
+    check(a.maxima, blocks * a.max_wgs * 16, "largest bounds");
+    check(a.tickets, blocks * 4, "tickets");
+    for (uint64_t i = 0; i < blocks; ++i)
       if (a.tickets[i] != 0) hipsim_fail("a ticket is not zero");
+    if ((uint64_t)a.max_wgs * kSelectPages < a.key_stride) hipsim_fail("workgroups do not cover the pages");
     for (uint32_t i = 0; i < a.chunks; ++i) {
       const PagedChunk& c = a.c[i];
       const uint32_t last = (c.start + c.rows - 1) >> a.kv.page_log2;
-      if (c.rows > a.max_rows || last >= a.key_stride || last >= max_pages) hipsim_fail("chunk past the launch's sizes");
+      if ((c.rows + a.rows_per_block - 1) / a.rows_per_block > a.max_blocks || last >= a.key_stride) hipsim_fail("chunk past the launch's sizes");
       if (a.raw) check_rotation(a.rot, c.start + c.rows - 1);
-      if (a.raw && a.group * (d + 4) > kSelectFloats) hipsim_fail("raw queries past the kernel's room");
+      if (a.raw && (c.rows != 1 || a.group * (d + 4) > kSelectFloats)) hipsim_fail("raw queries past the kernel's room");
       check(a.q + (uint64_t)c.row0 * a.num_heads * d, (uint64_t)c.rows * a.num_heads * d * 4, "q");
       check(a.pages + (uint64_t)c.row0 * a.kv.hkv * a.budget, (uint64_t)c.rows * a.kv.hkv * a.budget * 4, "selected pages");
       check_pages(a.kv, c.seq, 0, last, d, f16 ? 2 : 4);

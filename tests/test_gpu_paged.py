@@ -412,6 +412,51 @@ def test_selection_of_many_pages(hip, pages):
     kv.close()
 
 
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("case", ["zero", "tiny", "small", "large", "one", "nan", "inf", "equal", "near"])
+def test_selection_does_not_depend_on_rounding(hip, half, case):
+    """Scores that are equal, that differ in their last bits, that underflow or overflow 32 bits or are no
+    numbers: the pages are those of scores in 64 bits, ties to the lowest."""
+    hkv, d, n = 2, 64, 300
+    kv = hip.paged_kv_cache(1, n * 32, n, 32, hkv, d, half, 1, True)
+    kv.reserve(0, n * 32)
+    dt = np.float16 if half else np.float32
+    bounds = np.sort(synth.normal(5, "bounds", (n, hkv, 2, d)).astype(dt), axis=2)
+    q = synth.normal(5, "q", (3, 6, d)).astype(np.float32)
+    if case == "zero":
+        q[1] = 0.0
+    elif case in ("tiny", "small", "large"):
+        q = (q * np.float32({"tiny": 1e-38, "small": 1e-30, "large": 1e37}[case])).astype(np.float32)
+    elif case == "one":
+        q[:, :, 1:] = 0.0
+    elif case in ("nan", "inf"):
+        q[1, 4, 3] = np.float32(case)
+    elif case == "equal":
+        bounds[20:200] = bounds[20]
+    else:
+        bounds[20:200] = bounds[20]
+        for i in range(20, 200):
+            bounds[i, :, 1, i % d] += dt(2.0 ** -9 if half else 2.0 ** -22) * dt(i % 7)
+    rt.check(rt.hip().hipMemcpy(kv.storage(0).bounds, bounds.ctypes.data, bounds.nbytes, rt.H2D), "copy")
+    kv.set_length(0, 0, n * 32)
+    dq, sel = rt.DeviceArray.from_host(q.reshape(-1)), A.PageSelection(23, 2, 1)
+    out = rt.DeviceArray(3 * hkv * sel.budget, np.uint32)
+    hip.synchronize()
+    kv.select_device(A.AttentionLayer(0, 6), [(0, n * 32 - 3, 3)], sel, dq.ptr, dq.count, out.ptr, out.count)
+    hip.synchronize()
+    got, b = out.download().reshape(3, hkv, sel.budget), bounds.astype(np.float64)
+    for r in range(3):
+        for j in range(hkv):
+            x = q[r, 3 * j:3 * j + 3].astype(np.float64)
+            with np.errstate(invalid="ignore"):
+                score = np.maximum(x[:, None] * b[None, :, j, 0], x[:, None] * b[None, :, j, 1]).sum(-1).max(0)
+            score[np.isnan(score)] = np.inf
+            score[:2] = score[-1:] = np.inf
+            want = np.argsort(-score[2:n - 1], kind="stable")[:23] + 2
+            np.testing.assert_array_equal(got[r, j], np.concatenate([[0, 1], np.sort(want), [n - 1]]))
+    kv.close()
+
+
 def test_infinite_bounds_are_chosen(hip):
     """A page with an overflowed key counts as the highest, also where a zero of the query meets it."""
     s = Session(hip, 4, 2, 64, True, 32, [400], bounds=True)
