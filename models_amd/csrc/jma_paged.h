@@ -117,7 +117,7 @@ struct PagedSelectArgs {
   uint32_t* tickets;   // [block], zero between launches; block = (chunk, row block, kv head)
   uint32_t num_heads, group, top, first, last, budget;
   uint32_t rows_per_block, max_blocks;  // query rows of a workgroup; row blocks of the chunk with the most
-  uint32_t key_stride, max_wgs;  // pages, and workgroups, of the row furthest back
+  uint32_t key_stride, max_wgs;  // pages of the row furthest back; workgroups a block may have
   uint32_t chunks;
   PagedChunk c[kMaxChunks];
 };

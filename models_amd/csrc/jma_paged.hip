@@ -251,31 +251,43 @@ struct Keys {
   }
 };
 
-// Which of the bins of a histogram holds the need-th largest; then need is its rank within the bin.
+// Sum over this lane and the ones before it.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t lane_moved(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, kRows, 0xF, false);
+}
+__device__ __forceinline__ uint32_t sum_up_to(uint32_t x) {
+  x += lane_moved<0x111, 0xF>(x);  // row_shr by 1, 2, 4, 8
+  x += lane_moved<0x112, 0xF>(x);
+  x += lane_moved<0x114, 0xF>(x);
+  x += lane_moved<0x118, 0xF>(x);
+  x += lane_moved<0x142, 0xA>(x);  // lane 15 of a row to the next, then lane 31 to the upper half
+  x += lane_moved<0x143, 0xC>(x);
+  return x;
+}
+
+// Which of the 64 kPerLane bins of a histogram holds the need-th largest; then need is its rank within the bin.
 template <uint32_t kPerLane>
 __device__ __forceinline__ void border_bin(const uint32_t* hist, uint32_t lane, uint32_t& need, uint32_t& bin, uint32_t& count) {
+  const uint32_t b0 = kPerLane * (63 - lane);  // the highest bins first
   uint32_t c[kPerLane], mine = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < kPerLane; ++i) c[i] = hist[kPerLane * lane + i], mine += c[i];
-  uint32_t above = mine;
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    const uint32_t x = __shfl_down(above, m);
-    if (lane + m < 64) above += x;
+  for (uint32_t i = 0; i < kPerLane; i += 4) {
+    const uint4 x = *(const uint4*)&hist[b0 + i];
+    c[i] = x.x, c[i + 1] = x.y, c[i + 2] = x.z, c[i + 3] = x.w;
+    mine += x.x + x.y + x.z + x.w;
   }
-  uint32_t left = above - mine, b = 0, n = 0, rest = 0;  // entries of the bins above this lane's
-  bool found = false;
+  const uint32_t upto = sum_up_to(mine);
+  const int at = __ffsll((long long)__ballot(upto >= need)) - 1;
+  uint32_t left = upto - mine, b = 0, n = 0, rest = 0;
 #pragma unroll
   for (int i = (int)kPerLane - 1; i >= 0; --i) {
-    if (!found && left + c[i] >= need && left < need) {
-      found = true;
-      b = kPerLane * lane + i;
-      n = c[i];
-      rest = need - left;
-    }
+    const bool here = left < need && left + c[i] >= need;
+    b = here ? b0 + i : b;
+    n = here ? c[i] : n;
+    rest = here ? need - left : rest;
     left += c[i];
   }
-  const int at = __ffsll((long long)__ballot(found)) - 1;
   bin = __builtin_amdgcn_readlane(b, at);
   count = __builtin_amdgcn_readlane(n, at);
   need = __builtin_amdgcn_readlane(rest, at);
@@ -356,14 +368,14 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   const uint32_t rows = min(a.rows_per_block, c.rows - r0);
   const uint32_t pos0 = c.start + r0, row0 = c.row0 + r0;
   auto pages_of = [&](uint32_t r) JMA_INL { return ((pos0 + r) >> a.kv.page_log2) + 1; };
-  const uint32_t n1 = pages_of(rows - 1), first_page = blockIdx.x * kSelectPages;
-  if (first_page >= n1) return;
+  const uint32_t n1 = pages_of(rows - 1);
+  if (blockIdx.x * kSelectPages >= n1) return;
   auto list_of = [&](uint32_t r) JMA_INL { return a.pages + ((uint64_t)(row0 + r) * hkv + kvh) * a.budget; };
   if (blockIdx.x == 0)  // rows that see no more pages than they may
     for (uint32_t r = 0; r < rows && pages_of(r) <= a.budget; ++r)
       for (uint32_t i = threadIdx.x; i < a.budget; i += 256) list_of(r)[i] = i < pages_of(r) ? i : kNoPage;
   if (n1 <= a.budget) return;
-  const uint32_t wgs = (n1 + kSelectPages - 1) / kSelectPages;
+  const uint32_t wgs = min(gridDim.x, (n1 + kSelectPages - 1) / kSelectPages);
   const uint64_t block = ((uint64_t)blockIdx.z * a.max_blocks + blockIdx.y / hkv) * hkv + kvh;
   float* keys = a.keys + block * a.rows_per_block * 2 * a.key_stride;  // [row][2 key_stride]
   float* maxima = a.maxima + block * 4 * a.max_wgs;
@@ -371,7 +383,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   extern __shared__ __attribute__((aligned(16))) float s_queries[];  // raw: [group][D + 4]
   union Space {
     struct {
-      float q[16 * kQStride], score[kSelectPages][17], max[4];
+      float q[16 * kQStride], score[kSelectPages][17];
     };
     PickSpace pick;
   };
@@ -386,19 +398,6 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   const uint32_t* table = a.kv.table + (uint64_t)c.seq * a.kv.table_stride;
   auto bounds_of = [&](uint32_t p) JMA_INL { return (const KV*)a.kv.bounds + ((uint64_t)table[p] * hkv + kvh) * 2 * D; };
 
-  // This lane's share of 16 pages' bounds: page 16 wave + c16.
-  constexpr int kCh = kF16 ? D / 32 : D / 16;  // operands of either bound
-  typedef std::conditional_t<kF16, half8_t, float4_t> operand_t;
-  constexpr int kE = kF16 ? 8 : 4;
-  operand_t lo[kCh], hi[kCh];
-  {
-    const KV* b = bounds_of(min(first_page + 16 * wave + c16, n1 - 1)) + kE * g;
-#pragma unroll
-    for (int i = 0; i < kCh; ++i) {
-      lo[i] = *(const operand_t*)(b + 4 * kE * i);
-      hi[i] = *(const operand_t*)(b + D + 4 * kE * i);
-    }
-  }
   const float* q = a.q + ((uint64_t)row0 * a.num_heads + kvh * a.group) * D;
   if (a.raw) {
     for (uint32_t i = tid; i < a.group * (D / 4); i += 256)
@@ -408,6 +407,10 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   auto query = [&](uint32_t r, uint32_t h) JMA_INL -> const float* {
     return a.raw ? s_queries + h * kQStride : q + ((uint64_t)r * a.num_heads + h) * D;
   };
+  constexpr int kCh = kF16 ? D / 32 : D / 16;  // operands of a bound
+  typedef std::conditional_t<kF16, half8_t, float4_t> operand_t;
+  constexpr int kE = kF16 ? 8 : 4;
+  float most = 0.0f;
   for (uint32_t h0 = 0; h0 < a.group; h0 += 16) {
     const uint32_t heads = min(16u, a.group - h0);
     __syncthreads();
@@ -418,10 +421,9 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
       *(float4_t*)&s_q[col * kQStride + e] = x;
     }
     __syncthreads();
-    float factor = 1.0f, l1 = 0.0f;
-    float4_t s = {0.f, 0.f, 0.f, 0.f};
+    float factor = 1.0f, l1 = 0.0f, top = 0.0f;
+    int ex = 0;
     const float* mine = s_q + c16 * kQStride + kE * g;
-    float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < kCh; ++i)
 #pragma unroll
@@ -431,71 +433,80 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
         top = fmaxf(top, x);
       }
     l1 = sum_groups(l1);
+    l1 = l1 < INFINITY ? l1 : INFINITY;  // also where it is no number
+    if (wave == 0 && g == 0) s_l1[c16] = h0 == 0 ? l1 : fmaxf(l1, s_l1[c16]);
     if constexpr (kF16) {
       top = max_groups(top);
-      int ex = 0;
       if (top > 0.0f && top < INFINITY) ex = __builtin_amdgcn_frexp_expf(top);
       ex = max(ex, -100);
       factor = __builtin_amdgcn_ldexpf(1.0f, ex - 14);
+    }
+    // 16 pages at a time.
+    for (uint32_t p16 = 16 * (4 * blockIdx.x + wave); p16 < n1; p16 += 64 * wgs) {
+      operand_t lo[kCh], hi[kCh];
+      const KV* b = bounds_of(min(p16 + c16, n1 - 1)) + kE * g;
 #pragma unroll
       for (int i = 0; i < kCh; ++i) {
-        half8_t below_h, below_l, above_h, above_l;
+        lo[i] = *(const operand_t*)(b + 4 * kE * i);
+        hi[i] = *(const operand_t*)(b + D + 4 * kE * i);
+      }
+      float4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = __builtin_amdgcn_ldexpf(mine[32 * i + e], 14 - ex);
-          _Float16 h, l;
-          halves(fminf(x, 0.0f), h, l);
-          below_h[e] = h;
-          below_l[e] = l;
-          halves(fmaxf(x, 0.0f), h, l);
-          above_h[e] = h;
-          above_l[e] = l;
+      for (int i = 0; i < kCh; ++i) {
+        if constexpr (kF16) {
+          half8_t below_h, below_l, above_h, above_l;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x = __builtin_amdgcn_ldexpf(mine[32 * i + e], 14 - ex);
+            _Float16 h, l;
+            halves(fminf(x, 0.0f), h, l);
+            below_h[e] = h;
+            below_l[e] = l;
+            halves(fmaxf(x, 0.0f), h, l);
+            above_h[e] = h;
+            above_l[e] = l;
+          }
+          s = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[i], below_l, s, 0, 0, 0);
+          s = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[i], above_l, s, 0, 0, 0);
+          s = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[i], below_h, s, 0, 0, 0);
+          s = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[i], above_h, s, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = mine[16 * i + e];
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(lo[i][e], fminf(x, 0.0f), s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(hi[i][e], fmaxf(x, 0.0f), s, 0, 0, 0);
+          }
         }
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[i], below_l, s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[i], above_l, s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[i], below_h, s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[i], above_h, s, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) most = fmaxf(most, fmaxf(fabsf((float)lo[i][e]), fabsf((float)hi[i][e])));
       }
-    } else {
+      // Lane (g, c) holds pages 4g .. 4g + 3 of column c. A score that is not finite stays so.
+      float(*score)[17] = s_mem.score + 16 * wave;
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int i = 0; i < kCh; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = mine[16 * i + e];
-          s = __builtin_amdgcn_mfma_f32_16x16x4f32(lo[i][e], fminf(x, 0.0f), s, 0, 0, 0);
-          s = __builtin_amdgcn_mfma_f32_16x16x4f32(hi[i][e], fmaxf(x, 0.0f), s, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) score[4 * g + i][c16] = s[i] * factor;
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (p16 + c16 < n1)
+        for (uint32_t r = g; r < rows; r += 4) {
+          float best = -INFINITY;
+          bool odd = false;
+          for (uint32_t h = 0; h < heads; ++h) {
+            const float x = score[c16][r * heads + h];
+            odd = odd || !(fabsf(x) < INFINITY);
+            best = fmaxf(best, x);
+          }
+          float* key = keys + (uint64_t)r * 2 * a.key_stride + p16 + c16;
+          if (h0 > 0) {  // this lane's own
+            const float x = __hip_atomic_load(key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            odd = odd || x != x;
+            best = fmaxf(best, x);
+          }
+          __hip_atomic_store(key, odd ? NAN : best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-    }
-    // Lane (g, c) holds pages 4g .. 4g + 3 of column c. A score that is not finite stays so.
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s_mem.score[16 * wave + 4 * g + i][c16] = s[i] * factor;
-    l1 = l1 < INFINITY ? l1 : INFINITY;  // also where it is no number
-    if (wave == 0 && g == 0) s_l1[c16] = h0 == 0 ? l1 : fmaxf(l1, s_l1[c16]);
-    __syncthreads();
-    for (uint32_t i = tid; i < kSelectPages * rows; i += 256) {
-      const uint32_t p = first_page + i % kSelectPages, r = i / kSelectPages;
-      float best = -INFINITY;
-      bool odd = false;
-      for (uint32_t h = 0; h < heads; ++h) {
-        const float x = s_mem.score[i % kSelectPages][r * heads + h];
-        odd = odd || !(fabsf(x) < INFINITY);
-        best = fmaxf(best, x);
-      }
-      if (p >= n1) continue;
-      float* key = keys + (uint64_t)r * 2 * a.key_stride + p;
-      if (h0 > 0) {
-        const float x = __hip_atomic_load(key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        odd = odd || x != x;
-        best = fmaxf(best, x);
-      }
-      __hip_atomic_store(key, odd ? NAN : best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
-  float most = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kCh; ++i)
-#pragma unroll
-    for (int e = 0; e < kE; ++e) most = fmaxf(most, fmaxf(fabsf((float)lo[i][e]), fabsf((float)hi[i][e])));
   most = max_wave(most);
   if (lane == 0) __hip_atomic_store(&maxima[4 * blockIdx.x + wave], most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // The keys are acknowledged (visible device-wide) before the ticket is taken.
@@ -512,6 +523,9 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   auto exact = [&](uint32_t r, uint32_t p) JMA_INL -> uint64_t {
     constexpr int kX = D / 16;
     const KV* b = bounds_of(p) + c16 * kX;
+    float low[kX], high[kX];
+#pragma unroll
+    for (int e = 0; e < kX; ++e) low[e] = (float)b[e], high[e] = (float)b[D + e];
     double best = -INFINITY;
     bool odd = false;
     for (uint32_t h = 0; h < a.group; ++h) {
@@ -519,9 +533,8 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
       double s = 0.0;
 #pragma unroll
       for (int e = 0; e < kX; ++e) {
-        const float low = (float)b[e], high = (float)b[D + e];
-        s = fma((double)x[e], (double)(x[e] > 0.0f ? high : low), s);
-        if (x[e] == 0.0f) s = fma((double)x[e], (double)high, s);  // either infinity against a zero counts
+        s = fma((double)x[e], (double)(x[e] > 0.0f ? high[e] : low[e]), s);
+        if (x[e] == 0.0f) s = fma((double)x[e], (double)high[e], s);  // either infinity against a zero counts
       }
       s = row_sum(s);
       odd = odd || s != s;
@@ -531,7 +544,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   };
   // The pages of row r, by a wave of its own, or by all four.
   auto pick = [&](uint32_t r, auto team) JMA_INL {
-    constexpr uint32_t kWaves = decltype(team)::value, kBins = kWaves * kPickBins;
+    constexpr uint32_t kWaves = decltype(team)::value, kBins = kWaves == 1 ? kPickBins : 2 * kPickBins, kZero = kBins / kWaves;
     const uint32_t m = kWaves == 1 ? 0 : wave, w = wave - m;  // which of the team; its first wave, whose share of the LDS it has
     auto meet = [&]() JMA_INL {
       if constexpr (kWaves > 1) {
@@ -559,7 +572,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
     float bound = 0.0f;  // the largest of the pages' bounds
     for (uint32_t i = lane; i < 4 * wgs; i += 64) bound = fmaxf(bound, __hip_atomic_load(&maxima[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 #pragma unroll
-    for (uint32_t i = 0; i < kPickBins / 64; ++i) hist[kPickBins * m + 64 * i + lane] = 0;
+    for (uint32_t i = 0; i < kZero / 64; ++i) hist[kZero * m + 64 * i + lane] = 0;
     float least = INFINITY, most = -INFINITY;
     bool odd = false;
     for (uint32_t b = p0; b < p1; b += 512) {
@@ -612,19 +625,20 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
     const float eps = 1.001f * (0x1p-22f + (4 * D + 16) * 0x1p-23f) * l1 * bound + 0x1p-120f;  // and underflows
     // Everything is scored in 64 bits where a score, or the steps of the histogram, are out of range.
     const bool all = odds != 0 || !(l1 < INFINITY) || !(eps < INFINITY) || !(most - least > 0x1p-90f && most - least < INFINITY);
-    const float steps = (float)(kBins - 1) / (most - least), off = 2.0f * eps;
-    auto bin_of = [&](float x) JMA_INL { return min((uint32_t)fmaxf((x - least) * steps, 0.0f), kBins - 1); };
-    uint32_t bin = 0;
+    float high = INFINITY, low = -INFINITY;  // above: taken; below: not
     if (!all) {
+      const float steps = (float)(kBins - 1) / (most - least), step = (most - least) / (float)(kBins - 1);
       each([&](uint32_t, float x, bool there) JMA_INL {
-        if (there) atomicAdd(&hist[bin_of(x)], 1u);
+        if (there) atomicAdd(&hist[min((uint32_t)((x - least) * steps), kBins - 1)], 1u);
       });
       meet();
-      uint32_t need = a.top, count;
+      uint32_t need = a.top, bin, count;
       border_bin<kBins / 64>(hist, lane, need, bin, count);
+      high = least + ((float)bin + 1.01f) * step + 2.0f * eps;  // .01: (x - least) * steps is rounded
+      low = least + ((float)bin - 0.01f) * step - 2.0f * eps;
     }
-    auto above = [&](float x) JMA_INL { return !all && bin_of(x - off) > bin; };
-    auto near = [&](float x) JMA_INL { return all || (bin_of(x - off) <= bin && bin_of(x + off) >= bin); };
+    auto above = [&](float x) JMA_INL { return x > high; };
+    auto near = [&](float x) JMA_INL { return !(x > high) && !(x < low); };
     uint32_t sure = 0, count = 0;
     if (!all) {
       each([&](uint32_t p, float x, bool there) JMA_INL {

@@ -344,7 +344,6 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, h
     check(a.tickets, blocks * 4, "tickets");
     for (uint64_t i = 0; i < blocks; ++i)
       if (a.tickets[i] != 0) hipsim_fail("a ticket is not zero");
-    if ((uint64_t)a.max_wgs * kSelectPages < a.key_stride) hipsim_fail("workgroups do not cover the pages");
     for (uint32_t i = 0; i < a.chunks; ++i) {
       const PagedChunk& c = a.c[i];
       const uint32_t last = (c.start + c.rows - 1) >> a.kv.page_log2;
