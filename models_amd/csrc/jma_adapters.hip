@@ -208,11 +208,9 @@ __global__ __launch_bounds__(512) void adapter_down_kernel(const AdapterArgs a) 
       load(ya, w0);
       for (uint32_t c = w0;; c += 128) {
         load(yb, c + 64);
-        __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead of the products
         products(ya, c);
         if (c + 64 >= w1) break;
         load(ya, c + 128);
-        __builtin_amdgcn_sched_barrier(0);
         products(yb, c + 64);
         if (c + 128 >= w1) break;
       }

@@ -24,14 +24,17 @@ namespace {
 
 // Workgroup = (storage tile of 32 slots that a chunk writes to, head of q, k or v, chunk). The rows'
 // parts of that head go through LDS: one thread a row forms a head's norm sum in the reference's
-// order, pairs are rotated in place, and keys and values are stored in the page's layout. Bound by
-// latency for single tokens and by the bytes of q, k and v for prompts.
+// order, pairs are rotated, and keys and values are stored in the page's layout. All that a workgroup reads
+// (rows, factors of their positions, norm weight) is in flight before the first is used: one memory round
+// trip, which bounds it up to some hundred rows, and the bytes of q, k and v beyond (2048 rows of 32 + 16
+// heads of 128: APPEND_FIGURES; read piece by piece it took 24).
 template <typename KV, int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs a) {
   const PagedChunk c = a.c[blockIdx.z];
   if (c.rows == 0) return;
-  const uint32_t tile = c.start / kTileSlots + blockIdx.x;
-  const uint32_t p0 = max(c.start, tile * kTileSlots), p1 = min(c.start + c.rows, (tile + 1) * kTileSlots);
+  constexpr uint32_t kT = paged_append_rows(D);
+  const uint32_t tile = c.start / kT + blockIdx.x;
+  const uint32_t p0 = max(c.start, tile * kT), p1 = min(c.start + c.rows, (tile + 1) * kT);
   if (p0 >= p1) return;
   const uint32_t n = p1 - p0;
   const uint32_t hkv = a.kv.hkv;
@@ -46,30 +49,59 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
   src += (row0 * heads + head) * D;
 
   constexpr int kStride = D + 4;
-  __shared__ __attribute__((aligned(16))) float s_x[kTileSlots][kStride];
-  __shared__ float s_scale[kTileSlots];
-  for (uint32_t i = threadIdx.x; i < n * (D / 4); i += 256) {
-    const uint32_t r = i / (D / 4), e = 4 * (i % (D / 4));
-    *(float4_t*)&s_x[r][e] = *(const float4_t*)(src + (uint64_t)r * heads * D + e);
-  }
-  __syncthreads();
+  __shared__ __attribute__((aligned(16))) float s_x[kT][kStride];
+  __shared__ float s_scale[kT];
+  const uint32_t tid = threadIdx.x;
+  constexpr uint32_t kLoads = kT * (D / 4) / 256, kRows = 256 / (D / 4);  // rows of 256 pieces of 16 bytes
+  constexpr uint32_t kPairs = kT * (D / 2) / 256, kPairRows = 256 / (D / 2);
+  const bool rotates = (is_q || is_k) && a.rot.cos_t != nullptr && a.rot.pairs > 0;
   const float* w = is_q ? a.rot.q_norm_w : is_k ? a.rot.k_norm_w : nullptr;
   const bool v_norm = !is_q && !is_k && a.rot.v_norm != 0;
+  float4_t x[kLoads];
+  float cs[kPairs], sn[kPairs], weight = 1.0f;
+  const uint32_t row = tid / (D / 4), e4 = 4 * (tid % (D / 4)), pair_row = tid / (D / 2), pair = tid % (D / 2);
+#pragma unroll
+  for (uint32_t i = 0; i < kLoads; ++i)
+    if (kRows * i < n) x[i] = *(const float4_t*)(src + (uint64_t)min(row + kRows * i, n - 1) * heads * D + e4);
+  if (rotates) {
+    const uint64_t at = (uint64_t)p0 * a.rot.pairs + min(pair, a.rot.pairs - 1);
+#pragma unroll
+    for (uint32_t i = 0; i < kPairs; ++i)
+      if (kPairRows * i < n) {
+        const uint64_t f = at + (uint64_t)min(pair_row + kPairRows * i, n - 1) * a.rot.pairs;
+        cs[i] = a.rot.cos_t[f];
+        sn[i] = a.rot.sin_t[f];
+      }
+  }
+  if (w != nullptr) weight = w[tid % D];
+#pragma unroll
+  for (uint32_t i = 0; i < kLoads; ++i)
+    if (row + kRows * i < n) *(float4_t*)&s_x[row + kRows * i][e4] = x[i];
+  __syncthreads();
   if (w != nullptr || v_norm) {
 #pragma clang fp contract(off)
-    if (threadIdx.x < n) s_scale[threadIdx.x] = head_scale<D>(s_x[threadIdx.x], a.rot.norm_eps, v_norm);
+    if (tid < n) s_scale[tid] = head_scale<D>(s_x[tid], a.rot.norm_eps, v_norm);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n * D; i += 256) {
-      const uint32_t r = i / D, e = i % D;
-      float x = s_x[r][e] * s_scale[r];
-      if (!v_norm) x = x * w[e];
-      s_x[r][e] = x;
+    for (uint32_t r = tid / D; r < n; r += 256 / D) {
+      float y = s_x[r][tid % D] * s_scale[r];
+      if (!v_norm) y = y * weight;
+      s_x[r][tid % D] = y;
     }
     __syncthreads();
   }
-  if ((is_q || is_k) && a.rot.cos_t != nullptr) {
-    for (uint32_t i = threadIdx.x; i < n * a.rot.pairs; i += 256)
-      rotate_in(s_x[i / a.rot.pairs], i % a.rot.pairs, a.rot, p0 + i / a.rot.pairs);
+  if (rotates) {
+    const uint32_t e0 = a.rot.neox ? pair : 2 * pair, e1 = a.rot.neox ? pair + a.rot.pairs : 2 * pair + 1;
+    if (pair < a.rot.pairs) {
+#pragma unroll
+      for (uint32_t i = 0; i < kPairs; ++i) {
+        const uint32_t r = pair_row + kPairRows * i;
+        if (r >= n) break;
+        float x0 = s_x[r][e0], x1 = s_x[r][e1];
+        rotate_pair(x0, x1, cs[i], sn[i]);
+        s_x[r][e0] = x0;
+        s_x[r][e1] = x1;
+      }
+    }
     __syncthreads();
   }
   if (is_q) {
@@ -101,15 +133,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
   } else {
     KV* dst = (KV*)a.kv.v + base + (slot0 / kTileSlots) * kTileSlots * D;
     const uint32_t at = slot0 % kTileSlots;
-    if (n == kTileSlots) {
+    if (n == kT) {
       constexpr uint32_t kW = kF16 ? 8 : 4;
-      for (uint32_t i = threadIdx.x; i < kTileSlots / kW * D; i += 256) {
-        const uint32_t e = i / (kTileSlots / kW), r = (i % (kTileSlots / kW)) * kW;
+      for (uint32_t i = threadIdx.x; i < kT / kW * D; i += 256) {
+        const uint32_t e = i / (kT / kW), r = (i % (kT / kW)) * kW;
         typedef KV kv16_t __attribute__((ext_vector_type(kW)));
         kv16_t y;
 #pragma unroll
         for (uint32_t t = 0; t < kW; ++t) y[t] = (KV)s_x[r + t][e];
-        *(kv16_t*)(dst + e * kTileSlots + r) = y;
+        *(kv16_t*)(dst + e * kTileSlots + at + r) = y;
       }
     } else {
       for (uint32_t i = threadIdx.x; i < n * D; i += 256) {

@@ -320,7 +320,7 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, bool f16, uint32_t d, h
     for (uint32_t i = 0; i < a.chunks; ++i) {
       const PagedChunk& c = a.c[i];
       const uint32_t last = c.start + c.rows - 1;
-      if (last / kTileSlots - c.start / kTileSlots >= a.max_tiles) hipsim_fail("chunk of more tiles than the grid");
+      if (last / paged_append_rows(d) - c.start / paged_append_rows(d) >= a.max_tiles) hipsim_fail("chunk of more tiles than the grid");
       if ((last >> a.kv.page_log2) - (c.start >> a.kv.page_log2) >= a.max_pages) hipsim_fail("chunk of more pages than the grid");
       const uint64_t qd = (uint64_t)a.num_heads * d, kd = (uint64_t)a.kv.hkv * d;
       if (a.q_out) {
