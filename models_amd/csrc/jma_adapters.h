@@ -25,6 +25,7 @@ JMA_HD uint64_t adapter_b_index(uint64_t out, uint32_t r, uint32_t outs) {
 // `rows` rows from row0 on, adapter at element offsets a_at, b_at of the weights (rank16 0: none).
 struct AdapterRun {
   uint32_t rows, row0, rank16;
+  uint32_t block0;  // blocks of kUpRows rows of the launch's runs before this one
   float scale;
   uint64_t a_at, b_at;
 };
@@ -40,7 +41,7 @@ struct AdapterArgs {
   uint32_t dtype, cols, outs, max_rank16;
   uint32_t splits, cols_per_split;  // pieces of the columns in the two-launch form
   uint32_t row_block;               // rows of one workgroup in the one-launch form
-  uint32_t max_rows, runs;
+  uint32_t max_rows, runs, blocks;  // blocks: of kUpRows rows, of all runs
   AdapterRun run[kMaxRuns];
 };
 static_assert(sizeof(AdapterArgs) <= 4096, "kernel arguments exceed their limit");
@@ -63,7 +64,7 @@ JMA_HD uint32_t adapter_few_rows(uint32_t cols) {
 // Rows and outputs of a workgroup's tile in the two-launch form.
 constexpr uint32_t kDownRows = 16, kUpRows = 32, kUpOuts = 128;
 // Pieces of the columns: as many as keep the first product's workgroups (one a compute unit) in one round,
-// at least 512 columns each.
+// at least 512 columns each. row_blocks: of kDownRows rows.
 inline uint32_t adapter_splits(uint32_t cols, uint64_t row_blocks, uint32_t cus) {
   const uint64_t want = cus / std::max<uint64_t>(row_blocks, 1);
   return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({want, 16ull, std::max(1u, cols / 512)}));

@@ -48,6 +48,19 @@ struct Raw {
   }
 };
 
+// The run that a block of rows belongs to: a grid of the runs' blocks one after another, none empty, so that
+// workgroups spread evenly (three runs of 500 to 900 rows, a grid of the longest's blocks for each: some
+// compute units got two workgroups, others none, 29 us for the first product instead of ADAPTERS_DOWN_GRID).
+__device__ __forceinline__ const AdapterRun& run_of(const AdapterArgs& a, uint32_t block) {
+  uint32_t lo = 0, hi = a.runs;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (a.run[mid].block0 <= block) lo = mid;
+    else hi = mid;
+  }
+  return a.run[lo];
+}
+
 template <int kCtrl>
 __device__ __forceinline__ float moved(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), kCtrl, 0xF, 0xF, false));
@@ -159,8 +172,9 @@ __global__ __launch_bounds__(512) void adapter_few_kernel(const AdapterArgs a) {
 // adapters.
 template <uint32_t kType>
 __global__ __launch_bounds__(512) void adapter_down_kernel(const AdapterArgs a) {
-  const AdapterRun run = a.run[blockIdx.z];
-  const uint32_t r0 = blockIdx.y * kDownRows;
+  constexpr uint32_t kPer = kUpRows / kDownRows;
+  const AdapterRun run = run_of(a, blockIdx.y / kPer);
+  const uint32_t r0 = (blockIdx.y - run.block0 * kPer) * kDownRows;
   if (run.rank16 == 0 || r0 >= run.rows) return;
   const uint32_t rows = min(kDownRows, run.rows - r0);
   const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
@@ -244,9 +258,8 @@ __global__ __launch_bounds__(512) void adapter_down_kernel(const AdapterArgs a) 
 // 512 bytes. Bound by those.
 template <uint32_t kType>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterArgs a) {
-  const AdapterRun run = a.run[blockIdx.z];
-  const uint32_t r0 = blockIdx.y * kUpRows;
-  if (r0 >= run.rows) return;
+  const AdapterRun run = run_of(a, blockIdx.y);
+  const uint32_t r0 = (blockIdx.y - run.block0) * kUpRows;
   const uint32_t rows = min(kUpRows, run.rows - r0);
   const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15, wave = threadIdx.x >> 6;
   const uint32_t o0 = blockIdx.x * kUpOuts;
@@ -368,8 +381,7 @@ hipError_t launch_adapter_few(const AdapterArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_adapter_long(const AdapterArgs& a, hipStream_t stream) {
-  const dim3 down(a.splits, (a.max_rows + kDownRows - 1) / kDownRows, a.runs);
-  const dim3 up((a.outs + kUpOuts - 1) / kUpOuts, (a.max_rows + kUpRows - 1) / kUpRows, a.runs);
+  const dim3 down(a.splits, a.blocks * (kUpRows / kDownRows)), up((a.outs + kUpOuts - 1) / kUpOuts, a.blocks);
   return by_type(a.dtype, [&](auto type) {
     constexpr uint32_t kType = decltype(type)::value;
     if (a.max_rank16) adapter_down_kernel<kType><<<down, 512, 0, stream>>>(a);

@@ -467,8 +467,14 @@ hipError_t launch_adapter_few(const AdapterArgs& a, hipStream_t stream) {
 
 hipError_t launch_adapter_long(const AdapterArgs& a, hipStream_t stream) {
   return run(stream, "adapter_long_kernels", [a] {
-    check_grid(a.splits, (a.max_rows + kDownRows - 1) / kDownRows, a.runs);
-    check_grid((a.outs + kUpOuts - 1) / kUpOuts, (a.max_rows + kUpRows - 1) / kUpRows, a.runs);
+    check_grid(a.splits, a.blocks * (kUpRows / kDownRows), 1);
+    check_grid((a.outs + kUpOuts - 1) / kUpOuts, a.blocks, 1);
+    uint32_t blocks = 0;
+    for (uint32_t i = 0; i < a.runs; ++i) {
+      if (a.run[i].block0 != blocks) hipsim_fail("runs' blocks are not one after another");
+      blocks += (a.run[i].rows + kUpRows - 1) / kUpRows;
+    }
+    if (blocks != a.blocks) hipsim_fail("blocks of the runs");
     if ((uint64_t)a.splits * a.cols_per_split < a.cols || (uint64_t)(a.splits - 1) * a.cols_per_split >= a.cols)
       hipsim_fail("pieces do not cover the columns");
     check_runs(a, true);
