@@ -62,7 +62,7 @@ JMA_HD uint32_t adapter_few_rows(uint32_t cols) {
   return fit < 4u ? fit : 4u;
 }
 // Rows and outputs of a workgroup's tile in the two-launch form.
-constexpr uint32_t kDownRows = 16, kUpRows = 32, kUpOuts = 128;
+constexpr uint32_t kDownRows = 16, kUpRows = 16, kUpOuts = 128;
 // Pieces of the columns: as many as keep the first product's workgroups (one a compute unit) in one round,
 // at least 512 columns each. row_blocks: of kDownRows rows.
 inline uint32_t adapter_splits(uint32_t cols, uint64_t row_blocks, uint32_t cus) {

@@ -252,7 +252,7 @@ __global__ __launch_bounds__(512) void adapter_down_kernel(const AdapterArgs a) 
   }
 }
 
-// Workgroup = (128 outputs, 32 rows of a run, run): base + scale B (A x), the pieces of A x summed in order
+// Workgroup = (128 outputs, 16 rows of a run): base + scale B (A x), the pieces of A x summed in order
 // into LDS first. A wave takes 32 outputs; a 16x16x4 product leaves lane (g, c) four neighbouring outputs
 // of row c, which go through LDS, so that base is read (before all else) and out written in whole rows of
 // 512 bytes. Bound by those.
