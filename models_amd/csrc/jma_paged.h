@@ -51,6 +51,7 @@ JMA_HD uint32_t paged_v_index(uint32_t slot, uint32_t e, uint32_t d) {
 // nsplit splits, whose states are items part0 + (block of the chunk) * nsplit + split.
 struct PagedChunk {
   uint32_t seq, start, rows, row0, nsplit, part0;
+  uint32_t block0;  // 16-column attention: blocks of rows of the launch's chunks before this one
 };
 
 // What new rows are made with: QK-norm, then RoPE.
@@ -98,6 +99,7 @@ struct PagedAttendArgs {
   uint32_t rows_per_block;  // query rows of one workgroup
   uint32_t rows_per_stripe, heads_per_stripe;  // prefill: query rows and heads of a wave's 32 columns
   uint32_t max_blocks;   // row blocks of the chunk with the most
+  uint32_t blocks;       // and of all chunks (16-column attention)
   uint32_t tiles_per_split, max_splits;
   uint32_t chunks;
   PagedChunk c[kMaxChunks];
@@ -164,7 +166,7 @@ JMA_HD void paged_range(uint32_t pos0, uint32_t pos1, uint32_t window, uint32_t 
 // wave, raised until the launch is near `target` workgroups and no block needs more than kMaxSplits
 // splits. Fills the chunks' nsplit and part0.
 struct PagedPlan {
-  uint32_t tiles_per_split = 0, max_splits = 1, max_blocks = 0, rows_per_block = 1, head_groups = 1;
+  uint32_t tiles_per_split = 0, max_splits = 1, max_blocks = 0, blocks = 0, rows_per_block = 1, head_groups = 1;
   uint64_t part_bytes = 0, ticket_bytes = 0;
 };
 inline PagedPlan plan_paged(PagedChunk* c, uint32_t chunks, uint32_t group, uint32_t hkv, uint32_t d, bool f16,
@@ -189,7 +191,10 @@ inline PagedPlan plan_paged(PagedChunk* c, uint32_t chunks, uint32_t group, uint
       total += n * per;
       longest = std::max(longest, n);
     });
-    p.max_blocks = std::max(p.max_blocks, (c[i].rows + p.rows_per_block - 1) / p.rows_per_block);
+    const uint32_t blocks = (c[i].rows + p.rows_per_block - 1) / p.rows_per_block;
+    p.max_blocks = std::max(p.max_blocks, blocks);
+    c[i].block0 = p.blocks;
+    p.blocks += blocks;
   }
   uint64_t tps = std::max<uint64_t>(waves, (total + target - 1) / std::max(target, 1u));
   tps = std::max<uint64_t>(tps, (longest + kMaxSplits - 1) / kMaxSplits);
@@ -205,7 +210,7 @@ inline PagedPlan plan_paged(PagedChunk* c, uint32_t chunks, uint32_t group, uint
   }
   if (p.max_splits > 1) {
     p.part_bytes = items * kHeadSlots * (d + 4) * 4;
-    p.ticket_bytes = (uint64_t)chunks * p.max_blocks * per * 4;
+    p.ticket_bytes = (uint64_t)p.blocks * per * 4;
   }
   return p;
 }

@@ -903,11 +903,22 @@ void paged_attend_kernel(const PagedAttendArgs a) {
   __shared__ float s_scale[18];
   __shared__ uint32_t s_ticket;
 
-  const PagedChunk ch = a.c[blockIdx.z];
   const uint32_t hkv = a.kv.hkv, R = a.rows_per_block;
-  const uint32_t kvh = blockIdx.y % hkv, rest = blockIdx.y / hkv;
+  const uint32_t block = blockIdx.y / (hkv * a.head_groups);
+  uint32_t chunk = block;
+  if (!kFused && a.max_blocks > 1) {  // the chunk that this block of rows belongs to
+    uint32_t lo = 0, hi = a.chunks;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (a.c[mid].block0 <= block) lo = mid;
+      else hi = mid;
+    }
+    chunk = lo;
+  }
+  const PagedChunk ch = a.c[chunk];
+  const uint32_t nth = blockIdx.y - ch.block0 * hkv * a.head_groups;  // among the chunk's
+  const uint32_t kvh = nth % hkv, rest = nth / hkv;
   const uint32_t hg = rest % a.head_groups, row0 = rest / a.head_groups * R;
-  if (row0 >= ch.rows) return;
   const uint32_t rows = min(R, ch.rows - row0), heads = min(16u, a.group - 16 * hg);
   const uint32_t pos0 = ch.start + row0, pos1 = pos0 + rows - 1;
 
@@ -1244,8 +1255,8 @@ void paged_attend_kernel(const PagedAttendArgs a) {
   __syncthreads();
 
   const uint32_t cols = rows * heads;
-  const uint64_t unit = (uint64_t)blockIdx.z * gridDim.y + blockIdx.y;
-  float* part = a.part + (ch.part0 + (uint64_t)blockIdx.y * ch.nsplit) * (16 * (D + 4));  // this block's states
+  const uint32_t unit = blockIdx.y;
+  float* part = a.part + (ch.part0 + (uint64_t)nth * ch.nsplit) * (16 * (D + 4));  // this block's states
   const __amdgpu_buffer_rsrc_t rs = part_rsrc(part);
   float* out = a.out + (qrow * a.num_heads + kvh * a.group + 16 * hg) * D;
   auto finish = [&](uint32_t c, uint32_t e, const float4_t& o, float sum) JMA_INL {
@@ -1360,7 +1371,7 @@ hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, h
     using KV = decltype(kv);
     constexpr int D = decltype(dim)::value;
     const bool fused = a.k_new != nullptr;
-    const dim3 grid(a.max_splits + (fused ? 1 : 0), a.max_blocks * a.kv.hkv * a.head_groups, a.chunks);
+    const dim3 grid(a.max_splits + (fused ? 1 : 0), a.blocks * a.kv.hkv * a.head_groups);
     constexpr uint32_t kThreads = 64 * paged_waves(D);
     if (fused && a.pages != nullptr) paged_attend_kernel<KV, D, true, true><<<grid, kThreads, 0, stream>>>(a);
     else if (fused) paged_attend_kernel<KV, D, false, true><<<grid, kThreads, 0, stream>>>(a);

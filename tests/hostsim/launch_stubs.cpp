@@ -359,15 +359,19 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, h
 
 hipError_t launch_paged_attend(const PagedAttendArgs& a, bool f16, uint32_t d, hipStream_t stream) {
   return run(stream, "paged_attend_kernel", [a, f16, d] {
-    const uint64_t units = (uint64_t)a.max_blocks * a.kv.hkv * a.head_groups;
-    check_grid(a.max_splits, units, a.chunks);
+    const uint64_t units = (uint64_t)a.blocks * a.kv.hkv * a.head_groups;
+    check_grid(a.max_splits, units, 1);
     if (a.max_splits > 1) {
-      check(a.tickets, units * a.chunks * 4, "tickets");
-      for (uint64_t i = 0; i < units * a.chunks; ++i)
+      check(a.tickets, units * 4, "tickets");
+      for (uint64_t i = 0; i < units; ++i)
         if (a.tickets[i] != 0) hipsim_fail("a ticket is not zero");
     }
+    uint32_t before = 0;
     for (uint32_t i = 0; i < a.chunks; ++i) {
       const PagedChunk& c = a.c[i];
+      if (c.block0 != before) hipsim_fail("chunks' blocks are not one after another");
+      before += (c.rows + a.rows_per_block - 1) / a.rows_per_block;
+      if (before > a.blocks || (a.max_blocks == 1 && c.rows > a.rows_per_block)) hipsim_fail("chunk past the grid");
       const uint64_t qd = (uint64_t)a.num_heads * d;
       check(a.q + c.row0 * qd, c.rows * qd * 4, "q");
       check(a.out + c.row0 * qd, c.rows * qd * 4, "out");
