@@ -1,5 +1,5 @@
 // Arguments and layout of the low-rank adapter kernels (jma_adapters.hip), shared with the host runtime
-// (jma_runtime_adapters.inc) and the CPU checks (tests/paged_check.cpp). Plain C++: no HIP types.
+// (jma_runtime_adapters.inc) and the CPU checks (tests/hostsim/launch_stubs.cpp). Plain C++: no HIP types.
 #pragma once
 
 #include <stdint.h>

@@ -1,5 +1,5 @@
 // Arguments, layout and launch planning of the paged-cache kernels (jma_paged.hip), shared with the
-// host runtime (jma_runtime_paged.inc) and the CPU checks (tests/paged_check.cpp). Plain C++: no HIP
+// host runtime (jma_runtime_paged.inc) and the CPU checks (tests/hostsim/launch_stubs.cpp). Plain C++: no HIP
 // types, so it also builds with g++ alone.
 #pragma once
 

@@ -27,7 +27,7 @@ namespace {
 // order, pairs are rotated, and keys and values are stored in the page's layout. All that a workgroup reads
 // (rows, factors of their positions, norm weight) is in flight before the first is used: one memory round
 // trip, which bounds it up to some hundred rows, and the bytes of q, k and v beyond (2048 rows of 32 + 16
-// heads of 128: APPEND_FIGURES; read piece by piece it took 24).
+// heads of 128: 20 us, 4.5 TB/s; read piece by piece it took 24).
 template <typename KV, int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs a) {
   const PagedChunk c = a.c[blockIdx.z];
@@ -386,10 +386,11 @@ __device__ __forceinline__ uint64_t nth_largest(Keys& keys, uint32_t n, uint32_t
 // again in 64 bits, where the products are exact (one or two of a thousand pages). Where they are more
 // than 64, or a bound is infinite, all pages of the row are.
 //
-// 16 pages' table entries and bounds are in flight before the first is used: the kernel's time is those
-// two memory round trips, the keys' way to the last workgroup of the block to finish, and its pick (a wave
-// a row). Scored in 64 bits throughout it took 45 us for 61 rows of 12 heads of 128 over 626 pages,
-// SELECT_FIGURES.
+// A wave takes 16 pages at a time, all their bounds in flight. One token of 32 heads of 64 over 1563 pages:
+// 14 us, of which the bounds and their products 2.6, the scores' way to the last workgroup of the block
+// to finish and its reading them 3.5, the pick (by its four waves) 5, the start and the lists' stores the
+// rest: dependent round trips throughout, no unit busy. 61 rows of 12 heads of 128 over 626 pages (a wave
+// picks a row) 25 us; scored in 64 bits throughout it was 45, and 17 for the token.
 template <typename KV, int D>
 __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs a) {
   constexpr bool kF16 = std::is_same<KV, _Float16>::value;
@@ -482,6 +483,8 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
         lo[i] = *(const operand_t*)(b + 4 * kE * i);
         hi[i] = *(const operand_t*)(b + D + 4 * kE * i);
       }
+      // The pages that are taken in any case are not scored; a new token's own may have no bounds yet.
+      const bool candidate = p16 + c16 >= a.first && p16 + c16 + a.last < n1;
       float4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kCh; ++i) {
@@ -510,8 +513,10 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
             s = __builtin_amdgcn_mfma_f32_16x16x4f32(hi[i][e], fmaxf(x, 0.0f), s, 0, 0, 0);
           }
         }
+        float here = 0.0f;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) most = fmaxf(most, fmaxf(fabsf((float)lo[i][e]), fabsf((float)hi[i][e])));
+        for (int e = 0; e < kE; ++e) here = fmaxf(here, fmaxf(fabsf((float)lo[i][e]), fabsf((float)hi[i][e])));
+        most = fmaxf(most, candidate ? here : 0.0f);
       }
       // Lane (g, c) holds pages 4g .. 4g + 3 of column c. A score that is not finite stays so.
       float(*score)[17] = s_mem.score + 16 * wave;
@@ -861,7 +866,7 @@ __device__ __forceinline__ void store_token(const PagedView& kv, const PagedChun
   if (kv.bounds != nullptr) page_bounds<KV, D, kThreads>(kv, page, kvh, slot + 1, key, s_red);
 }
 
-// Workgroup = (split, kv head x head group x block of query rows, chunk): 16 matrix-core columns =
+// Workgroup = (split, kv head x head group x block of query rows of a chunk): 16 matrix-core columns =
 // (query row, query head) pairs that share every K/V load; its waves stride over the split's steps
 // of 32 slots (f16) or 16 (f32), each with the running maximum and sum of its own softmax.
 //
@@ -883,6 +888,12 @@ __device__ __forceinline__ void store_token(const PagedView& kv, const PagedChun
 // step that a column sees in part, reaches all of the wave's columns (0 x inf is no 0); a wave with such an
 // output does its steps again, with those values taken out of the product and what they make of the
 // columns that see them (NaN) put in.
+//
+// Large batches are bound by the bytes of K and V (64 tokens of 32 + 8 heads of 128, 383 MB: 81 us, 4.7 TB/s,
+// where a large copy moves 5.2); one token by the dependent round trips from its table entry to the joined
+// splits (32 + 8 heads of 64, 700 positions: 9 us); f32 caches of many rows by f32
+// matrix instructions at half their rate, two waves a SIMD being what the registers hold (12 tokens and 200
+// rows of 16 + 8 heads of 128: 86 us). Eight waves a workgroup at heads of 128 took 89 us for the batch.
 template <typename KV, int D, bool kSelected, bool kFused>
 __global__ __launch_bounds__(64 * paged_waves(D)) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D == 128 ? 2 : 1)))
 void paged_attend_kernel(const PagedAttendArgs a) {
