@@ -109,6 +109,15 @@ def test_prompts(hip, dtype, rows):
     ad.set.close()
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_many_prompts(hip, dtype):
+    """More runs of many rows than a launch takes, of lengths around a block of rows."""
+    ad = Adapters(hip, 264, 133, [4, 33, 16, 70], dtype)
+    ad.check([(i % 4 if i % 9 else A.NO_ADAPTER, 9 + 5 * i % 27) for i in range(120)])
+    ad.check([(i % 4, 16 * (1 + i % 2) + i % 3 - 1) for i in range(50)], base=None)
+    ad.set.close()
+
+
 def test_many_runs(hip):
     ad = Adapters(hip, 256, 96, [4, 8, 12, 16, 20], A.ADAPTER_F16)
     ad.check([(i % 5 if i % 7 else A.NO_ADAPTER, i % 4) for i in range(400)])

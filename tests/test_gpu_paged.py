@@ -227,6 +227,19 @@ def test_chunks_of_many_sequences(hip, heads, hkv, d, half, page):
     s.close()
 
 
+@pytest.mark.parametrize("heads,hkv,d,half", [(8, 2, 64, True), (6, 2, 32, False), (4, 4, 128, True)])
+@pytest.mark.parametrize("sel", [None, A.PageSelection(2, 1, 1)])
+def test_more_chunks_than_a_launch_holds(hip, heads, hkv, d, half, sel):
+    """150 sequences of 1 to 20 new rows, whose blocks of rows lie one after another in the launches' grids,
+    single tokens beside prompts that need several blocks."""
+    n = 150
+    s = Session(hip, heads, hkv, d, half, 32, [200] * n, bounds=True)
+    s.fill([(i, 0, 1 + 37 * i % 150) for i in range(n)])
+    rows = [1 if i % 3 else 1 + 7 * i % 20 for i in range(n)]
+    s.run([(i, 1 + 37 * i % 150, rows[i]) for i in reversed(range(n))], "many", sel)
+    s.close()
+
+
 @pytest.mark.parametrize("neox,rotary", [(False, None), (True, 32), (False, 16), (True, 0)])
 def test_rotations(hip, neox, rotary):
     for half in (True, False):
@@ -409,6 +422,40 @@ def test_selection_of_many_pages(hip, pages):
                 score = np.maximum(x[:, None] * b[None, :, j, 0], x[:, None] * b[None, :, j, 1]).sum(-1).max(0)
                 score[:1] = score[-2:] = np.inf
                 np.testing.assert_array_equal(got[r, j], np.sort(np.argsort(-score, kind="stable")[:sel.budget]))
+    kv.close()
+
+
+def test_selection_in_several_launches(hip):
+    """A prompt whose rows' scores take more than one launch may hold, and whose rows see page counts below,
+    at and above what a selection takes."""
+    hkv, d, pages, rows = 2, 32, 5000, 1000
+    n = pages * 32
+    kv = hip.paged_kv_cache(1, n, pages, 32, hkv, d, True, 1, True)
+    kv.reserve(0, n)
+    bounds = np.sort(synth.normal(4, "bounds", (pages, hkv, 2, d)).astype(np.float16), axis=2)
+    rt.check(rt.hip().hipMemcpy(kv.storage(0).bounds, bounds.ctypes.data, bounds.nbytes, rt.H2D), "copy")
+    kv.set_length(0, 0, n)
+    q = synth.normal(4, "q", (rows, 6 * d))
+    dq, sel = rt.DeviceArray.from_host(q), A.PageSelection(9, 2, 3)
+    out = rt.DeviceArray(rows * hkv * sel.budget, np.uint32)
+    b = bounds.astype(np.float64)
+    for start in (0, n - rows):
+        hip.synchronize()
+        kv.select_device(A.AttentionLayer(0, 6), [(0, start, rows)], sel, dq.ptr, dq.count, out.ptr, out.count)
+        hip.synchronize()
+        got = out.download().reshape(rows, hkv, sel.budget)
+        for r in (0, 1, 4, 5, 200, 447, 448, 449, 479, 480, 511, 512, 653, 654, 655, 816, 998, 999):
+            seen = (start + r) // 32 + 1
+            for j in range(hkv):
+                want = np.full(sel.budget, A.NO_PAGE, np.uint32)
+                if seen <= sel.budget:
+                    want[:seen] = np.arange(seen)
+                else:
+                    x = q.reshape(rows, 6, d)[r, 3 * j:3 * j + 3].astype(np.float64)
+                    score = np.maximum(x[:, None] * b[None, :seen, j, 0], x[:, None] * b[None, :seen, j, 1]).sum(-1).max(0)
+                    score[:2] = score[seen - 3:] = np.inf
+                    want = np.sort(np.argsort(-score, kind="stable")[:sel.budget])
+                np.testing.assert_array_equal(got[r, j], want, f"row {r} at {start}, kv head {j}")
     kv.close()
 
 
