@@ -21,7 +21,7 @@ typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 
 #define JMA_INL __attribute__((always_inline))
 
@@ -75,6 +75,83 @@ __device__ __forceinline__ float wave_sum(float x) {
   x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ uint32_t max_groups(uint32_t x) {  // over the lanes of a column of a 16-column product
+  auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max(r[0], r[1]);
+}
+
+// acc += W x over 64 columns: lane (g, c) holds columns 8g .. 8g+7 of either 32, of row c of x and of row
+// c of each 16-row tile of W, whose stored type the matrix instructions take. f16: x is carried as two halves
+// (x = hi + lo to 2^-22, or to 2^-39 of the 64 columns' largest), scaled by a power of two that puts that into
+// [2^13, 2^14); bf16: as three pieces of 8 bits, exactly; f32, and where an x is no finite number: one f32
+// product of four columns after another. 64 columns of 64 ranks: 1.8 us a pair of waves in f32, 0.2 in halves.
+template <uint32_t kType, int kN>
+__device__ __forceinline__ void products(const float (&x)[2][8], const Raw<kType, 8> (&w)[2][kN], float4_t (&acc)[kN]) {
+  if constexpr (kType != kAdapterF32) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
+    bits = max_groups(bits);
+    if (__ballot(bits >= 0x7F800000u) == 0) {
+      if constexpr (kType == kAdapterF16) {
+        const int ex = max(bits != 0 ? __builtin_amdgcn_frexp_expf(__uint_as_float(bits)) : 0, -100);
+        float4_t sum[kN] = {};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          half8_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = __builtin_amdgcn_ldexpf(x[i][e], 14 - ex);
+            hi[e] = (_Float16)y;
+            lo[e] = (_Float16)(y - (float)hi[e]);
+          }
+#pragma unroll
+          for (int n = 0; n < kN; ++n) sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, w[i][n].w), lo, sum[n], 0, 0, 0);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, w[i][n].w), hi, sum[n], 0, 0, 0);
+        }
+        const float factor = __builtin_amdgcn_ldexpf(1.0f, ex - 14);
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(sum[n][e], factor, acc[n][e]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float rest[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) rest[e] = x[i][e];
+#pragma unroll
+          for (int piece = 0; piece < 3; ++piece) {
+            uint4_t top;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const uint32_t a = __float_as_uint(rest[e]), b = __float_as_uint(rest[e + 1]);
+              top[e / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);  // their upper halves
+              rest[e] -= __uint_as_float(a & 0xFFFF0000u);
+              rest[e + 1] -= __uint_as_float(b & 0xFFFF0000u);
+            }
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+              acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8_t, w[i][n].w), __builtin_bit_cast(bf8_t, top), acc[n], 0, 0, 0);
+          }
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int n = 0; n < kN; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i][n][e], x[i][e], acc[n], 0, 0, 0);
 }
 
 // Workgroup = (512 outputs, block of kRows rows, run). Every workgroup forms all of A x for its rows: A
@@ -207,26 +284,35 @@ __global__ __launch_bounds__(512) void adapter_down_kernel(const AdapterArgs a) 
         for (int n = 0; n < kTiles; ++n) y.w[i][n].load(a.a, wrow + (uint64_t)16 * n * a.cols + at);
       }
     };
-    auto products = [&](Operands& y, uint32_t c) JMA_INL {
+    auto step = [&](Operands& y, uint32_t c) JMA_INL {
+      float v[2][8];
 #pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) {
-        const bool in = c + 32 * i + 8 * g < w1;
+      for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 8; ++e) v[i][e] = y.v[i][e / 4][e % 4];
+      if (c + 64 > w1) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+          const bool in = c + 32 * i + 8 * g < w1;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] = in ? v[i][e] : 0.0f;
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
-            acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? y.w[i][n][e] : 0.0f, in ? y.v[i][e / 4][e % 4] : 0.0f, acc[n], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < Raw<kType, 8>::kWords; ++e) y.w[i][n].w[e] = in ? y.w[i][n].w[e] : 0u;
+        }
       }
+      products<kType, kTiles>(v, y.w, acc);
     };
     Operands ya, yb;
     if (w0 < w1) {
       load(ya, w0);
       for (uint32_t c = w0;; c += 128) {
         load(yb, c + 64);
-        products(ya, c);
+        step(ya, c);
         if (c + 64 >= w1) break;
         load(ya, c + 128);
-        products(yb, c + 64);
+        step(yb, c + 64);
         if (c + 128 >= w1) break;
       }
     }
@@ -285,16 +371,16 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterArgs a) {
       for (uint32_t e = 0; e < 4; ++e)
         if (o + e < a.outs) base[i][e] = p[e];
   }
-  constexpr int kRowTiles = kUpRows / 16;
-  float4_t acc[kRowTiles][2] = {};  // [row tile][output tile]
+  static_assert(kUpRows == 16, "one tile of rows");
+  float4_t acc[2] = {};  // [output tile]
   for (uint32_t rank0 = 0; rank0 < run.rank16; rank0 += 64) {
     const uint32_t ranks = min(64u, run.rank16 - rank0);
-    Raw<kType, 4> w[4][2];
+    Raw<kType, 8> w[2][2];
 #pragma unroll
-    for (uint32_t k = 0; k < 4; ++k)
+    for (uint32_t k = 0; k < 2; ++k)
 #pragma unroll
       for (int n = 0; n < 2; ++n)
-        w[k][n].load(a.b, run.b_at + adapter_b_index(min(o0 + 32 * wave + 16 * n + c16, a.outs - 1), rank0 + min(16 * k, ranks - 16) + 4 * g, a.outs));
+        w[k][n].load(a.b, run.b_at + adapter_b_index(min(o0 + 32 * wave + 16 * n + c16, a.outs - 1), rank0 + min(32 * k + 8 * g, ranks - 8), a.outs));
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < kUpRows * (ranks / 4); i += 256) {
       const uint32_t row = i / (ranks / 4), r = 4 * (i % (ranks / 4));
@@ -306,24 +392,24 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterArgs a) {
       *(float4_t*)&s_mem[row * kDownStride + r] = sum * run.scale;
     }
     __syncthreads();
+    float d[2][8];
 #pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) {
-      if (16 * k >= ranks) break;
+    for (uint32_t k = 0; k < 2; ++k) {
+      const bool in = 32 * k + 8 * g < ranks;
+      const float* p = &s_mem[c16 * kDownStride + (in ? 32 * k + 8 * g : 0)];
+      const float4_t d0 = *(const float4_t*)p, d1 = *(const float4_t*)(p + 4);
 #pragma unroll
-      for (int t = 0; t < kRowTiles; ++t) {
-        const float4_t d = *(const float4_t*)&s_mem[(16 * t + c16) * kDownStride + 16 * k + 4 * g];
+      for (int e = 0; e < 4; ++e) d[k][e] = in ? d0[e] : 0.0f, d[k][4 + e] = in ? d1[e] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int n = 0; n < 2; ++n) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[k][n][e], d[e], acc[t][n], 0, 0, 0);
-      }
+        for (int e = 0; e < Raw<kType, 8>::kWords; ++e) w[k][n].w[e] = in ? w[k][n].w[e] : 0u;
     }
+    products<kType, 2>(d, w, acc);
   }
   __syncthreads();
 #pragma unroll
-  for (int t = 0; t < kRowTiles; ++t)
-#pragma unroll
-    for (int n = 0; n < 2; ++n) *(float4_t*)&s_mem[(16 * t + c16) * kOutStride + 32 * wave + 16 * n + 4 * g] = acc[t][n];
+  for (int n = 0; n < 2; ++n) *(float4_t*)&s_mem[c16 * kOutStride + 32 * wave + 16 * n + 4 * g] = acc[n];
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
