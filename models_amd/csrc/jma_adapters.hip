@@ -2,11 +2,12 @@
 // of rows with an adapter of its own.
 //
 //   adapter_few_kernel    runs of few rows, one launch: every workgroup forms all of A x for its rows
-//   adapter_down_kernel   longer runs: A x on the f32 matrix cores, split over the columns
-//   adapter_up_kernel     base + scale B (A x) on the f32 matrix cores
+//   adapter_down_kernel   longer runs: A x on the matrix cores, split over the columns
+//   adapter_up_kernel     base + scale B (A x) on the matrix cores
 //
-// Inputs, sums and outputs are 32-bit, weights are widened exactly, so the result is that of 32-bit
-// arithmetic for every weight type; sums are formed in a fixed order.
+// Inputs, sums and outputs are 32-bit and weights exact, so the result is that of 32-bit arithmetic for
+// every weight type (f16 weights of longer runs: inputs to 2^-22, below); sums are formed in a fixed order.
+// A weight that is no finite number may make NaN of what 32-bit arithmetic makes infinite.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -50,7 +51,7 @@ struct Raw {
 
 // The run that a block of rows belongs to: a grid of the runs' blocks one after another, none empty, so that
 // workgroups spread evenly (three runs of 500 to 900 rows, a grid of the longest's blocks for each: some
-// compute units got two workgroups, others none, 29 us for the first product instead of 18).
+// compute units got two workgroups, others none, 29 us for the first product instead of 18, in f32 products).
 __device__ __forceinline__ const AdapterRun& run_of(const AdapterArgs& a, uint32_t block) {
   uint32_t lo = 0, hi = a.runs;
   while (hi - lo > 1) {
@@ -243,17 +244,17 @@ __global__ __launch_bounds__(512) void adapter_few_kernel(const AdapterArgs a) {
 
 // Workgroup = (piece of the columns, 16 rows of a run): A x over that piece. Its eight waves take an
 // eighth of the piece each and meet in LDS, so that few pieces, which the second launch has to sum, fill
-// the device. One 16x16x4 product takes 16 ranks x 16 rows over four columns; lane (g, c) holds eight
-// neighbouring columns 8g .. 8g+7 of its row of either operand per step of 32, so both are read in wide
-// loads, two steps ahead; ranks are taken 64 at a time, which is all of them for most adapters. 2000 rows by
-// 4096 columns, ranks 48 and 64: 18 us, of which f32 matrix instructions 7 and the bytes of x 6; the rest is the
-// first loads' latency and the meeting, which four steps a wave do not hide.
+// the device. Lane (g, c) holds eight neighbouring columns 8g .. 8g+7 of its row of either operand per 32, so
+// both are read in wide loads, two steps of 64 ahead; ranks are taken 64 at a time, which is all of them for
+// most adapters. 2000 rows by 4096 columns, ranks 48 and 64: 17 us for 33 MB of x and, out of the L2s, 64 MB of A,
+// which every workgroup reads: four steps a wave do not hide the loads' latency. Workgroups of 32 rows
+// read half of A and spill (22 us).
 template <uint32_t kType>
 __global__ __launch_bounds__(512) void adapter_down_kernel(const AdapterArgs a) {
-  constexpr uint32_t kPer = kUpRows / kDownRows;
-  const AdapterRun run = run_of(a, blockIdx.y / kPer);
-  const uint32_t r0 = (blockIdx.y - run.block0 * kPer) * kDownRows;
-  if (run.rank16 == 0 || r0 >= run.rows) return;
+  static_assert(kDownRows == kUpRows, "the runs' blocks are those of both products");
+  const AdapterRun run = run_of(a, blockIdx.y);
+  const uint32_t r0 = (blockIdx.y - run.block0) * kDownRows;
+  if (run.rank16 == 0) return;
   const uint32_t rows = min(kDownRows, run.rows - r0);
   const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -340,10 +341,10 @@ __global__ __launch_bounds__(512) void adapter_down_kernel(const AdapterArgs a) 
 }
 
 // Workgroup = (128 outputs, 16 rows of a run): base + scale B (A x), the pieces of A x summed in order
-// into LDS first. A wave takes 32 outputs; a 16x16x4 product leaves lane (g, c) four neighbouring outputs
-// of row c, which go through LDS, so that base is read (before all else) and out written in whole rows of
-// 512 bytes. Bound by those, in two rounds of workgroups (2000 rows by 4096 outputs: 20 us, 3.2 TB/s; tiles
-// of 32 rows, whose registers leave fewer workgroups resident, 24).
+// into LDS first. A wave takes 32 outputs; a product leaves lane (g, c) four neighbouring outputs of row c,
+// which go through LDS, so that base is read (before all else) and out written in whole rows of 512 bytes.
+// Bound by those, in rounds of six workgroups a compute unit (2000 rows by 4096 outputs: 17 us, 3.9 TB/s; in
+// f32 products 20; tiles of 32 rows, whose registers leave fewer workgroups resident, 24).
 template <uint32_t kType>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterArgs a) {
   const AdapterRun run = run_of(a, blockIdx.y);
@@ -469,7 +470,7 @@ hipError_t launch_adapter_few(const AdapterArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_adapter_long(const AdapterArgs& a, hipStream_t stream) {
-  const dim3 down(a.splits, a.blocks * (kUpRows / kDownRows)), up((a.outs + kUpOuts - 1) / kUpOuts, a.blocks);
+  const dim3 down(a.splits, a.blocks), up((a.outs + kUpOuts - 1) / kUpOuts, a.blocks);
   return by_type(a.dtype, [&](auto type) {
     constexpr uint32_t kType = decltype(type)::value;
     if (a.max_rank16) adapter_down_kernel<kType><<<down, 512, 0, stream>>>(a);

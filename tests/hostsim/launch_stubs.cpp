@@ -471,7 +471,7 @@ hipError_t launch_adapter_few(const AdapterArgs& a, hipStream_t stream) {
 
 hipError_t launch_adapter_long(const AdapterArgs& a, hipStream_t stream) {
   return run(stream, "adapter_long_kernels", [a] {
-    check_grid(a.splits, a.blocks * (kUpRows / kDownRows), 1);
+    check_grid(a.splits, a.blocks, 1);
     check_grid((a.outs + kUpOuts - 1) / kUpOuts, a.blocks, 1);
     uint32_t blocks = 0;
     for (uint32_t i = 0; i < a.runs; ++i) {

@@ -4,6 +4,13 @@ projections and the paged attention.
 The bound: the inputs and weights are exact in 32 bits, products and sums are rounded in 32 bits, so an
 output is off by at most (cols + rank + 16) 2^-24 of the sum of its terms' magnitudes, scale |B| (|A| |x|),
 plus one rounding of the whole, 2^-24 (|base| + that sum).
+
+Runs of more than 8 rows with f16 weights carry x and A x as two f16 halves, each off by at most 2^-22 of its
+value: 4 2^-24 of the terms' magnitudes for either product. A term of the first product then passes at most
+min(cols, 64) + 1 + cols / 256 + min(7, cols / 32) + cols / 512 rounded sums (of its 64 columns, of its wave's
+steps, of the waves and of the pieces), cols + 3 at most; one of the second at most rank + 2 with the scale's
+rounding: 13 beside cols + rank, of the 16 above. (An element below 2^-17 of the largest of its 64 columns is
+off by 2^-39 of that one, whose own term is a 2^-24 more than 2^15 times larger: the rest of the 16.)
 """
 
 import numpy as np
