@@ -10,7 +10,7 @@ value: 4 2^-24 of the terms' magnitudes for either product. A term of the first 
 min(cols, 64) + 1 + cols / 256 + min(7, cols / 32) + cols / 512 rounded sums (of its 64 columns, of its wave's
 steps, of the waves and of the pieces), cols + 3 at most; one of the second at most rank + 2 with the scale's
 rounding: 13 beside cols + rank, of the 16 above. (An element below 2^-17 of the largest of its 64 columns is
-off by 2^-39 of that one, whose own term is a 2^-24 more than 2^15 times larger: the rest of the 16.)
+off by 2^-39 of that one, 2^-15 of what a 2^-24 of its term is: within the rest of the 16.)
 """
 
 import numpy as np
@@ -122,6 +122,28 @@ def test_many_prompts(hip, dtype):
     ad = Adapters(hip, 264, 133, [4, 33, 16, 70], dtype)
     ad.check([(i % 4 if i % 9 else A.NO_ADAPTER, 9 + 5 * i % 27) for i in range(120)])
     ad.check([(i % 4, 16 * (1 + i % 2) + i % 3 - 1) for i in range(50)], base=None)
+    ad.set.close()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("rows", [3, 40])
+def test_inputs_that_are_no_numbers_stay_in_their_rows(hip, dtype, rows):
+    ad = Adapters(hip, 520, 300, [5, 64], dtype)
+    x = synth.normal(23, "x", (2 * rows, 520))
+    x[1, 3], x[rows + 2, 519] = np.inf, np.nan
+    x[rows, :] *= np.float32(1e30)
+    x[rows + 1, :] *= np.float32(1e-30)
+    dx, out = rt.DeviceArray.from_host(x), rt.DeviceArray(2 * rows * 300)
+    hip.synchronize()
+    ad.set.apply_device([(0, rows), (1, rows)], dx.ptr, dx.count, 0, out.ptr, out.count)
+    hip.synchronize()
+    got = out.download().reshape(2 * rows, 300)
+    odd = [1, rows + 2]
+    assert not np.isfinite(got[odd]).any()
+    with np.errstate(invalid="ignore"):
+        want, size = ad.reference([(0, rows), (1, rows)], x, None)
+    rest = np.delete(np.arange(2 * rows), odd)
+    assert (np.abs(got[rest] - want[rest]) <= size[rest]).all()
     ad.set.close()
 
 
