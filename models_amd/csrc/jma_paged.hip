@@ -560,22 +560,32 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   auto exact = [&](uint32_t r, uint32_t p) JMA_INL -> uint64_t {
     constexpr int kX = D / 16;
     const KV* b = bounds_of(p) + c16 * kX;
+    constexpr uint32_t kHeads = D >= 256 ? 2 : 4;  // heads whose elements are read together
     float low[kX], high[kX];
 #pragma unroll
     for (int e = 0; e < kX; ++e) low[e] = (float)b[e], high[e] = (float)b[D + e];
     double best = -INFINITY;
     bool odd = false;
-    for (uint32_t h = 0; h < a.group; ++h) {
-      const float* x = query(r, h) + c16 * kX;
-      double s = 0.0;
+    for (uint32_t h0 = 0; h0 < a.group; h0 += kHeads) {
+      float x[kHeads][kX];
 #pragma unroll
-      for (int e = 0; e < kX; ++e) {
-        s = fma((double)x[e], (double)(x[e] > 0.0f ? high[e] : low[e]), s);
-        if (x[e] == 0.0f) s = fma((double)x[e], (double)high[e], s);  // either infinity against a zero counts
+      for (uint32_t i = 0; i < kHeads; ++i) {
+        const float* from = query(r, min(h0 + i, a.group - 1)) + c16 * kX;
+#pragma unroll
+        for (int e = 0; e < kX; ++e) x[i][e] = from[e];
       }
-      s = row_sum(s);
-      odd = odd || s != s;
-      best = s > best ? s : best;
+#pragma unroll
+      for (uint32_t i = 0; i < kHeads; ++i) {
+        double s = 0.0;
+#pragma unroll
+        for (int e = 0; e < kX; ++e) {
+          const double u = (double)x[i][e] * (double)low[e], v = (double)x[i][e] * (double)high[e];  // exact
+          s += u > v || u != u ? u : v;
+        }
+        s = row_sum(s);
+        odd = odd || s != s;
+        best = s > best ? s : best;
+      }
     }
     return odd ? 0xFFFFFFFFFFFFFFFFull : ordered(best);
   };
@@ -659,6 +669,11 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
     const uint32_t heads = min(16u, a.group);
     float l1 = 0.0f;
     for (uint32_t h = 0; h < heads; ++h) l1 = fmaxf(l1, s_l1[r * heads + h]);
+    if (odds == 0 && l1 == 0.0f) {  // every score is zero
+      if (m == 0)
+        for (uint32_t i = lane; i < a.top; i += 64) out[i] = a.first + i;
+      return;
+    }
     const float eps = 1.001f * (0x1p-22f + (4 * D + 16) * 0x1p-23f) * l1 * bound + 0x1p-120f;  // and underflows
     // Everything is scored in 64 bits where a score, or the steps of the histogram, are out of range.
     const bool all = odds != 0 || !(l1 < INFINITY) || !(eps < INFINITY) || !(most - least > 0x1p-90f && most - least < INFINITY);

@@ -460,7 +460,7 @@ def test_selection_in_several_launches(hip):
 
 
 @pytest.mark.parametrize("half", [True, False])
-@pytest.mark.parametrize("case", ["zero", "tiny", "small", "large", "one", "nan", "inf", "equal", "near"])
+@pytest.mark.parametrize("case", ["zero", "tiny", "small", "large", "one", "nan", "inf", "equal", "near", "infinite"])
 def test_selection_does_not_depend_on_rounding(hip, half, case):
     """Scores that are equal, that differ in their last bits, that underflow or overflow 32 bits or are no
     numbers: the pages are those of scores in 64 bits, ties to the lowest."""
@@ -480,6 +480,11 @@ def test_selection_does_not_depend_on_rounding(hip, half, case):
         q[1, 4, 3] = np.float32(case)
     elif case == "equal":
         bounds[20:200] = bounds[20]
+    elif case == "infinite":                   # no number among a page's keys, and keys that overflowed
+        bounds[50, :, 0, 5], bounds[50, :, 1, 5] = np.inf, -np.inf
+        bounds[60, :, 0, 6] = bounds[70, 0, 0, 7] = -np.inf
+        bounds[80, :, 1, 8] = np.inf
+        q[0, :, 6] = q[1, :, 8] = 0.0
     else:
         bounds[20:200] = bounds[20]
         for i in range(20, 200):
