@@ -116,8 +116,8 @@ struct PagedSelectArgs {
   PagedRotation rot;
   uint32_t raw;
   uint32_t* pages;     // out: [rows][hkv][budget]
-  float* keys;         // scratch [block][row of the block][2 key_stride]: scores in 32 bits, or in 64, as
-                       // ordered integers, where those are needed
+  float* keys;         // scratch [block][row of the block][paged_row_keys]: scores in 32 bits, and behind them,
+                       // where those are needed, in 64, as ordered integers
   float* maxima;       // scratch [block][max_wgs][4]: largest bound of a wave's pages
   uint32_t* tickets;   // [block], zero between launches; block = (chunk, row block, kv head)
   uint32_t num_heads, group, top, first, last, budget;
@@ -137,6 +137,8 @@ struct PagedTableArgs {
 };
 static_assert(sizeof(PagedTableArgs) <= 4096, "kernel arguments exceed their limit");
 
+// Floats of one row's scores: 32 bits a page, to an even number, and 64 a page.
+JMA_HD uint64_t paged_row_keys(uint32_t pages) { return ((pages + 1) & ~1u) + (uint64_t)2 * pages; }
 // Query rows of a selection workgroup: its matrix product has 16 columns.
 JMA_HD uint32_t select_rows(uint32_t group) { return group >= 16 ? 1u : 16u / group; }
 // Floats of a group's queries that the selection kernel stages where it takes them raw.

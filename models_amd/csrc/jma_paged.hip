@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
   if (n1 <= a.budget) return;
   const uint32_t wgs = min(gridDim.x, (n1 + kSelectPages - 1) / kSelectPages);
   const uint64_t block = ((uint64_t)blockIdx.z * a.max_blocks + blockIdx.y / hkv) * hkv + kvh;
-  float* keys = a.keys + block * a.rows_per_block * 2 * a.key_stride;  // [row][2 key_stride]
+  float* keys = a.keys + block * a.rows_per_block * paged_row_keys(a.key_stride);
   float* maxima = a.maxima + block * 4 * a.max_wgs;
 
   extern __shared__ __attribute__((aligned(16))) float s_queries[];  // raw: [group][D + 4]
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
             odd = odd || !(fabsf(x) < INFINITY);
             best = fmaxf(best, x);
           }
-          float* key = keys + (uint64_t)r * 2 * a.key_stride + p16 + c16;
+          float* key = keys + (uint64_t)r * paged_row_keys(a.key_stride) + p16 + c16;
           if (h0 > 0) {  // this lane's own
             const float x = __hip_atomic_load(key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             odd = odd || x != x;
@@ -609,7 +609,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
     }
     if (a.top == 0) return;
     out += a.first;
-    float* row_keys = keys + (uint64_t)r * 2 * a.key_stride;
+    float* row_keys = keys + (uint64_t)r * paged_row_keys(a.key_stride);
     // This wave's share of the candidates, kept in LDS where it fits.
     const uint32_t candidates = n - a.last - a.first, share = (candidates + 64 * kWaves - 1) / (64 * kWaves) * 64;
     const uint32_t p0 = a.first + min(m * share, candidates), p1 = a.first + min((m + 1) * share, candidates);
@@ -754,19 +754,13 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
       });
       return;
     }
-    // Keys of 64 bits for all that are near, over the scores: whose place is first read by every wave.
-    meet();
-    uint64_t* wide = (uint64_t*)row_keys;
-    if (m != 0) return;
-    Keys k{wide, a.first, a.first + candidates, lane};
-    // From the last page to the first: key p lies over scores 2p and 2p + 1.
-    for (uint32_t left = candidates; left > 0;) {
-      const uint32_t len = (left - 1) % 64 + 1, b = k.first + left - len;
-      const float v = __hip_atomic_load(&row_keys[min(b + lane, k.end - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const bool there = lane < len;
-      uint64_t in = __ballot(there && near(v));
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (there && !near(v)) __hip_atomic_store(&wide[b + lane], above(v) ? ~0ull : 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // Keys of 64 bits for all that are near, behind the scores: four pages of the wave's share at a time.
+    uint64_t* wide = (uint64_t*)(row_keys + ((a.key_stride + 1) & ~1u));
+    for (uint32_t b = p0; b < p1; b += 64) {
+      const float v = __hip_atomic_load(&row_keys[min(b + lane, p1 - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const bool there = b + lane < p1;
+      uint64_t in = __ballot(there && (all || near(v)));
+      if (there && !(all || near(v))) __hip_atomic_store(&wide[b + lane], above(v) ? ~0ull : 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       while (in != 0) {
         uint32_t at[4];
         uint32_t found = 0;
@@ -779,9 +773,11 @@ __global__ __launch_bounds__(256) void paged_select_kernel(const PagedSelectArgs
         const uint64_t e = exact(r, p);
         if (c16 == 0 && g < found) __hip_atomic_store(&wide[p], e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
-      left -= len;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    meet();
+    if (m != 0) return;
+    Keys k{wide, a.first, a.first + candidates, lane};
     const uint64_t border = nth_largest(k, a.top, space.hist[w]);
     uint32_t larger = 0;
     k.each([&](uint32_t, uint64_t x, bool there) JMA_INL { larger += (uint32_t)__popcll(__ballot(there && x > border)); });

@@ -339,7 +339,7 @@ hipError_t launch_paged_select(const PagedSelectArgs& a, bool f16, uint32_t d, h
   return run(stream, "paged_select_kernel", [a, f16, d] {
     check_grid(a.max_wgs, (uint64_t)a.max_blocks * a.kv.hkv, a.chunks);
     const uint64_t blocks = (uint64_t)a.chunks * a.max_blocks * a.kv.hkv;
-    check(a.keys, blocks * a.rows_per_block * 2 * a.key_stride * 4, "page scores");
+    check(a.keys, blocks * a.rows_per_block * paged_row_keys(a.key_stride) * 4, "page scores");
     check(a.maxima, blocks * a.max_wgs * 16, "largest bounds");
     check(a.tickets, blocks * 4, "tickets");
     for (uint64_t i = 0; i < blocks; ++i)
